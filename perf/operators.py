@@ -178,7 +178,8 @@ def _own_linear(s):
 
 def _own_loss(s):
     import minigrid_amd as mg
-    loss, stats = mg.policy_loss(s["x"], s["a"], s["old"], s["adv"], mask=s["mask"], ref_log_prob=s["ref"], clip=CLIP, kl_coef=KL, entropy_coef=ENTROPY)
+    loss, stats = mg.policy_loss(s["x"], s["a"], s["old"], s["adv"], mask=s["mask"], ref_log_prob=s["ref"], clip=CLIP,
+                                 kl_coef=0.0 if s["ref"] is None else KL, entropy_coef=ENTROPY)
     grad, = torch.autograd.grad(loss, [s["x"]], s["scale"])
     return {"loss": loss.detach(), "stats": stats, "dlogits": grad}
 
