@@ -14,3 +14,11 @@ from .wrappers import (DictObservationSpaceWrapper, FullyObsWrapper, ImgObsWrapp
                        ViewSizeWrapper)
 
 __version__ = "0.1.0"
+
+
+def __getattr__(name):
+    # the learning operators need torch, the environments do not: they are imported when they are first asked for
+    if name in ("linear", "policy_loss", "sample_actions", "advantages"):
+        from . import ops
+        return getattr(ops, name)
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

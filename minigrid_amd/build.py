@@ -44,6 +44,11 @@ for _g in ("rooms", "sentence", "roomgrid", "light"):
     for _r in ("pcg", "philox"):
         for _k in ("refill", "generate"):
             UNITS[f"mg_gen_{_g}_{_r}_{_k}.hip"] = _GEN
+# the learning operators (include/minigrid_ops.h): no kernel of the environments sees them
+_OPS = ["ops/mg_ops.h", os.path.join("..", "..", "include", "minigrid_ops.h"), ABI_HEADER]
+UNITS.update({"ops/mg_linear.hip": _OPS + ["ops/mg_linear.h"], "ops/mg_policy.hip": _OPS, "ops/mg_advantages.hip": _OPS})
+# no packed 32-bit float instructions in them: ordinary float code would be turned into them
+UNIT_FLAGS = {u: ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"] for u in UNITS if u.startswith("ops/")}
 # the slowest units (minutes) first, so that the pool does not end on one of them
 SOURCES = sorted(UNITS, key=lambda n: (not n.startswith(("mg_gen_rooms", "mg_gen_lane_")), not n.startswith("mg_gen_sentence")))
 HEADERS = sorted({h for deps in UNITS.values() for h in deps})
@@ -126,8 +131,8 @@ def _build_locked(force, verbose, missing_hipcc_ok, lib, extra_flags, extra_link
 
     def compile_one(src):
         mine = flag_units is None or src in flag_units
-        cflags = base_cflags + (list(extra_flags) if mine else [])
-        base = os.path.splitext(src)[0] + (tag if mine else "")
+        cflags = base_cflags + UNIT_FLAGS.get(src, []) + (list(extra_flags) if mine else [])
+        base = os.path.splitext(src)[0].replace("/", "_") + (tag if mine else "")
         obj, stamp = os.path.join(OBJDIR, base + ".o"), os.path.join(OBJDIR, base + ".hash")
         want = _hash_files([src] + UNITS[src], " ".join(cflags))
         if not force and os.path.exists(obj) and os.path.exists(stamp) and open(stamp).read().strip() == want:

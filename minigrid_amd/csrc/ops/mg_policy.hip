@@ -1,0 +1,551 @@
+// mg_policy.hip — the clipped policy loss with its gradient, and the draw of actions (include/minigrid_ops.h).
+//
+// A row's distribution enters through three sums around its largest logit m:  s = sum e^{l - m},  t = sum e^{l - m} (l - m); then log-sum-exp = m + log s,
+// entropy = log s - t / s.  Both are gathered in one pass over the logits, the maximum running along.  What the loss decides by (is the ratio
+// beyond the clipping border?) and what the draw decides by (where does the running sum pass u s?) is held in 64 bits: a value next to a border
+// falls on the side that the mathematics says.
+#include "mg_ops.h"
+
+namespace mgo {
+
+constexpr int SMALL_VOCAB = 64;          // up to here a lane owns a row
+constexpr float NEG_INF = -__builtin_inff();
+
+struct Saved { double lse; float dlp, entropy; };       // of a row, for the backward pass: 16 bytes
+static_assert(sizeof(Saved) == 16, "the header promises 16 bytes a row");
+
+struct LossArgs {
+  const void* logits; int64_t ld; const void* action; int32_t action_dtype;
+  const float *old_lp, *adv, *ref_lp; const uint8_t* mask;
+  double lo, hi, kl, ent;                // 1 - clip_lo, 1 + clip_hi, kl_coef, ent_coef
+  Saved* save;
+  int64_t rows, vocab;
+};
+
+template <class A> __device__ __forceinline__ int64_t action_of(const A& a, int64_t i) {
+  return a.action_dtype == MG_DT_U8 ? ((const uint8_t*)a.action)[i] : a.action_dtype == MG_DT_I32 ? ((const int32_t*)a.action)[i] : ((const int64_t*)a.action)[i];
+}
+
+struct Terms { double policy, kl, entropy, clipped, count; };
+
+// the loss terms of a row that counts, from its statistics
+__device__ __forceinline__ void row_terms(const LossArgs& a, int64_t i, double lse, double entropy, double chosen, Terms& sum) {
+  const double lp = chosen - lse, adv = a.adv[i], q = exp(lp - (double)a.old_lp[i]);
+  const bool clipped = adv >= 0.0 ? q > a.hi : q < a.lo;
+  const double policy = -(clipped ? (adv >= 0.0 ? a.hi : a.lo) : q) * adv;
+  double dlp = clipped ? 0.0 : -q * adv, kl = 0.0;
+  if (a.ref_lp) {
+    const double gap = (double)a.ref_lp[i] - lp, e = exp(gap);
+    kl = e - gap - 1.0;
+    dlp += a.kl * (1.0 - e);
+  }
+  if (a.save) a.save[i] = {lse, (float)dlp, (float)entropy};
+  sum.policy += policy; sum.kl += kl; sum.entropy += entropy; sum.clipped += clipped ? 1.0 : 0.0; sum.count += 1.0;
+}
+
+__device__ __forceinline__ void write_out(const LossArgs& a, const Terms& t, float* out) {
+  const double inv = t.count > 0.0 ? 1.0 / t.count : 0.0, p = t.policy * inv, k = t.kl * inv, h = t.entropy * inv;
+  out[0] = (float)(p + a.kl * k - a.ent * h); out[1] = (float)p; out[2] = (float)k; out[3] = (float)h; out[4] = (float)(t.clipped * inv); out[5] = (float)t.count;
+}
+
+__device__ __forceinline__ void wave_sum(Terms& t) {
+  t.policy = wave_sum(t.policy); t.kl = wave_sum(t.kl); t.entropy = wave_sum(t.entropy); t.clipped = wave_sum(t.clipped); t.count = wave_sum(t.count);
+}
+
+// the workgroups' sums in their order (each lane its run of them, then the lanes): one workgroup
+__global__ __launch_bounds__(256) void k_loss_out(LossArgs a, int64_t n, const Terms* part, float* out) {
+  __shared__ Terms s[4];
+  Terms t = {};
+  for (int64_t u = threadIdx.x; u < n; u += 256) {
+    const Terms& p = part[u];
+    t.policy += p.policy; t.kl += p.kl; t.entropy += p.entropy; t.clipped += p.clipped; t.count += p.count;
+  }
+  wave_sum(t);
+  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = t;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    Terms r = {};
+    for (int w = 0; w < 4; w++) { r.policy += s[w].policy; r.kl += s[w].kl; r.entropy += s[w].entropy; r.clipped += s[w].clipped; r.count += s[w].count; }
+    write_out(a, r, out);
+  }
+}
+
+// `rows` rows of logits into LDS, row stride vocab | 1 (odd: a lane per row reads without bank conflicts), read as they lie in memory
+template <class T>
+__device__ __forceinline__ void stage_rows(const T* logits, int64_t ld, int64_t first, int rows, int vocab, float* lds) {
+  const int n = rows * vocab;
+  for (int u = threadIdx.x; u < n; u += blockDim.x) {
+    const int r = u / vocab, c = u - r * vocab;
+    lds[r * (vocab | 1) + c] = (float)logits[(first + r) * ld + c];
+  }
+}
+
+// few columns: a lane owns a row, 64-bit throughout (seven exponentials a row are nothing)
+template <class T>
+__global__ void k_loss_small(LossArgs a, Terms* part, float* out) {
+  extern __shared__ float lds[];
+  const int vocab = (int)a.vocab, R = blockDim.x;
+  const int64_t first = (int64_t)blockIdx.x * R;
+  const int rows = (int)min((int64_t)R, a.rows - first);
+  stage_rows((const T*)a.logits, a.ld, first, rows, vocab, lds);
+  __syncthreads();
+  Terms sum = {};
+  const int64_t i = first + threadIdx.x;
+  if ((int)threadIdx.x < rows && (!a.mask || a.mask[i])) {
+    const float* l = lds + threadIdx.x * (vocab | 1);
+    float m = NEG_INF;
+    for (int c = 0; c < vocab; c++) m = fmaxf(m, l[c]);
+    double s = 0.0, t = 0.0;
+    for (int c = 0; c < vocab; c++) {
+      const double d = (double)l[c] - (double)m, e = exp(d);
+      s += e;
+      t += e == 0.0 ? 0.0 : e * d;                              // a closed column: e^-inf (-inf) counts 0
+    }
+    const double ls = log(s);
+    const int64_t act = action_of(a, i);
+    row_terms(a, i, (double)m + ls, ls - t / s, act >= 0 && act < vocab ? (double)l[act] : __builtin_nan(""), sum);
+  }
+  // the workgroup's sums; LDS is free again
+  wave_sum(sum);
+  Terms* w = (Terms*)lds;
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    Terms r = {};
+    for (int v = 0; v < R / 64; v++) { r.policy += w[v].policy; r.kl += w[v].kl; r.entropy += w[v].entropy; r.clipped += w[v].clipped; r.count += w[v].count; }
+    if (gridDim.x == 1) write_out(a, r, out);
+    else part[blockIdx.x] = r;
+  }
+}
+
+// ---- long rows ----
+struct Sums { float m; double s, t; };
+
+__device__ __forceinline__ void join(Sums& a, float m, double s, double t) {      // a += (m, s, t)
+  const float M = fmaxf(a.m, m);
+  const double da = a.m == NEG_INF ? 0.0 : (double)a.m - (double)M, db = m == NEG_INF ? 0.0 : (double)m - (double)M;      // (a part without a finite logit has s = t = 0)
+  const double fa = exp(da), fb = exp(db);
+  a.t = fa * (a.t + da * a.s) + fb * (t + db * s);
+  a.s = fa * a.s + fb * s;
+  a.m = M;
+}
+
+template <int N>
+__device__ __forceinline__ void add_chunk(Sums& a, const float (&x)[N]) {
+  float top = x[0];
+#pragma unroll
+  for (int u = 1; u < N; u++) top = fmaxf(top, x[u]);
+  if (top > a.m) {
+    if (a.s != 0.0) {
+      const double d = (double)a.m - (double)top, f = exp(d);
+      a.t = f * (a.t + d * a.s);
+      a.s = f * a.s;
+    }
+    a.m = top;
+  }
+  if (a.m == NEG_INF) {                                          // nothing but -inf so far; a NaN must not get lost
+#pragma unroll
+    for (int u = 0; u < N; u++)
+      if (x[u] != x[u]) a.s = a.t = __builtin_nan("");
+    return;
+  }
+  float s = 0.0f, t = 0.0f;                                      // eight terms in 32 bits, then into the 64-bit sum
+#pragma unroll
+  for (int u = 0; u < N; u++) {
+    float d = x[u] - a.m;
+    d = d < -200.0f ? -200.0f : d;                               // e^-200 is 0 in 32 bits, and 0 * -200 is 0 (keeps a NaN)
+    const float e = __builtin_amdgcn_exp2f(d * LOG2E_HI);
+    s += e;
+    t = __builtin_fmaf(e, d, t);
+  }
+  a.s += (double)s;
+  a.t += (double)t;
+}
+
+template <class T> struct Pack { static constexpr int N = 16 / sizeof(T); };
+
+// the sums of elements [from, to) of a row over NT lanes
+template <class T, int NT>
+__device__ __forceinline__ Sums row_sums(const T* row, int64_t from, int64_t to, int tid) {
+  constexpr int N = Pack<T>::N;
+  Sums a = {NEG_INF, 0.0, 0.0};
+  const int64_t skew = (int64_t)(((uintptr_t)(row + from) & 15) / sizeof(T));
+  const int64_t head = min(to, from + (skew ? N - skew : 0)), body = head + (to - head) / N * N;
+  if (from + tid < head) { const float x[1] = {(float)row[from + tid]}; add_chunk(a, x); }
+  for (int64_t c = head + (int64_t)tid * N; c < body; c += (int64_t)NT * N) {
+    T v[N];
+    __builtin_memcpy(v, __builtin_assume_aligned(row + c, 16), 16);
+    float x[N];
+#pragma unroll
+    for (int u = 0; u < N; u++) x[u] = (float)v[u];
+    add_chunk(a, x);
+  }
+  if (body + tid < to) { const float x[1] = {(float)row[body + tid]}; add_chunk(a, x); }
+  return a;
+}
+
+__device__ __forceinline__ void wave_join(Sums& a) {
+  const float M = wave_max(a.m);
+  const double d = a.m == NEG_INF ? 0.0 : (double)a.m - (double)M, f = exp(d);
+  a.t = wave_sum(f * (a.t + d * a.s));
+  a.s = wave_sum(f * a.s);
+  a.m = M;
+}
+
+// a workgroup per row
+template <class T>
+__global__ __launch_bounds__(256) void k_loss_rows(LossArgs a, Terms* part) {
+  __shared__ Sums w[4];
+  const int64_t i = blockIdx.x;
+  Terms sum = {};
+  if (!a.mask || a.mask[i]) {                                    // (uniform in the workgroup)
+    const T* row = (const T*)a.logits + i * a.ld;
+    Sums s = row_sums<T, 256>(row, 0, a.vocab, threadIdx.x);
+    wave_join(s);
+    if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int v = 1; v < 4; v++) join(s, w[v].m, w[v].s, w[v].t);
+      const double ls = log(s.s);
+      const int64_t act = action_of(a, i);
+      row_terms(a, i, (double)s.m + ls, ls - s.t / s.s, act >= 0 && act < a.vocab ? (double)(float)row[act] : __builtin_nan(""), sum);
+    }
+  }
+  if (threadIdx.x == 0) part[i] = sum;
+}
+
+// d loss / d logit_j = g / count (dlp (1[j = action] - p_j) + ent p_j (l_j - lse + H)), p_j = e^{l_j - lse}
+struct GradArgs {
+  const void* logits; int64_t ld; const void* action; int32_t action_dtype; const uint8_t* mask;
+  const Saved* save; const float *out, *grad; void* dlogits;
+  float ent; int64_t rows, vocab;
+};
+__device__ __forceinline__ float grad_of(float l, double lse, float entropy, float dlp, float ent, bool chosen) {
+  float d = (float)((double)l - lse);
+  d = d < -200.0f ? -200.0f : d;
+  const float p = __builtin_amdgcn_exp2f(d * LOG2E_HI);
+  return p * (ent * (d + entropy) - dlp) + (chosen ? dlp : 0.0f);
+}
+
+template <class T>
+__global__ void k_grad_small(GradArgs a) {
+  extern __shared__ float lds[];
+  const int vocab = (int)a.vocab, R = blockDim.x;
+  const int64_t first = (int64_t)blockIdx.x * R;
+  const int rows = (int)min((int64_t)R, a.rows - first);
+  stage_rows((const T*)a.logits, a.ld, first, rows, vocab, lds);
+  __syncthreads();
+  if ((int)threadIdx.x < rows) {
+    float* l = lds + threadIdx.x * (vocab | 1);
+    const int64_t i = first + threadIdx.x;
+    if (!a.mask || a.mask[i]) {
+      const Saved s = a.save[i];
+      const float share = a.grad[0] / a.out[5], dlp = s.dlp * share, ent = a.ent * share;
+      const int64_t act = action_of(a, i);
+      for (int c = 0; c < vocab; c++) l[c] = grad_of(l[c], s.lse, s.entropy, dlp, ent, c == act);
+    } else {
+      for (int c = 0; c < vocab; c++) l[c] = 0.0f;
+    }
+  }
+  __syncthreads();
+  T* d = (T*)a.dlogits + first * vocab;
+  for (int u = threadIdx.x; u < rows * vocab; u += R) {
+    const int r = u / vocab, c = u - r * vocab;
+    d[u] = (T)lds[r * (vocab | 1) + c];
+  }
+}
+
+constexpr int64_t GRAD_RUN = 16384;      // elements of a row per workgroup
+
+template <class T>
+__global__ __launch_bounds__(256) void k_grad_rows(GradArgs a) {
+  constexpr int N = Pack<T>::N;
+  const int64_t i = blockIdx.x, from = (int64_t)blockIdx.y * GRAD_RUN, to = min(a.vocab, from + GRAD_RUN);
+  const bool on = !a.mask || a.mask[i];
+  const T* row = (const T*)a.logits + i * a.ld;
+  T* d = (T*)a.dlogits + i * a.vocab;
+  Saved s = {0.0, 0.0f, 0.0f};
+  float dlp = 0.0f, ent = 0.0f;
+  int64_t act = -1;
+  if (on) {
+    s = a.save[i];
+    const float share = a.grad[0] / a.out[5];
+    dlp = s.dlp * share; ent = a.ent * share; act = action_of(a, i);
+  }
+  // whole 16-byte stores: the run is counted from the gradient's alignment, the logits may lie at any
+  const int64_t skew = (int64_t)(((uintptr_t)(d + from) & 15) / sizeof(T));
+  const int64_t head = min(to, from + (skew ? N - skew : 0)), body = head + (to - head) / N * N;
+  auto one = [&](int64_t c) { d[c] = on ? (T)grad_of((float)row[c], s.lse, s.entropy, dlp, ent, c == act) : (T)0.0f; };
+  if (from + threadIdx.x < head) one(from + threadIdx.x);
+  for (int64_t c = head + (int64_t)threadIdx.x * N; c < body; c += 256 * N) {
+    T v[N] = {};
+    if (on) {
+      __builtin_memcpy(v, row + c, 16);
+#pragma unroll
+      for (int u = 0; u < N; u++) v[u] = (T)grad_of((float)v[u], s.lse, s.entropy, dlp, ent, c + u == act);
+    }
+    __builtin_memcpy(__builtin_assume_aligned(d + c, 16), v, 16);
+  }
+  if (body + threadIdx.x < to) one(body + threadIdx.x);
+}
+
+// ---- the draw ----
+__device__ __forceinline__ void store_action(void* action, int64_t vocab, int64_t i, int64_t k) {
+  if (vocab <= 256) ((uint8_t*)action)[i] = (uint8_t)k;
+  else ((int32_t*)action)[i] = (int32_t)k;
+}
+
+template <class T>
+__global__ void k_sample_small(const T* logits, int64_t ld, int64_t rows_all, int vocab, const float* u, void* action, float* lp) {
+  extern __shared__ float lds[];
+  const int R = blockDim.x;
+  const int64_t first = (int64_t)blockIdx.x * R;
+  const int rows = (int)min((int64_t)R, rows_all - first);
+  stage_rows(logits, ld, first, rows, vocab, lds);
+  __syncthreads();
+  if ((int)threadIdx.x >= rows) return;
+  const int64_t i = first + threadIdx.x;
+  const float* l = lds + threadIdx.x * (vocab | 1);
+  float m = NEG_INF;
+  int best = 0;
+  for (int c = 0; c < vocab; c++)
+    if (l[c] > m) { m = l[c]; best = c; }
+  double s = 0.0;
+  for (int c = 0; c < vocab; c++) s += exp((double)l[c] - (double)m);
+  int k = best;
+  if (u) {
+    const double target = (double)u[i] * s;
+    double run = 0.0;
+    int last = 0;
+    k = -1;
+    for (int c = 0; c < vocab && k < 0; c++) {
+      const double e = exp((double)l[c] - (double)m);
+      run += e;
+      if (e > 0.0) { last = c; if (run > target) k = c; }
+    }
+    if (k < 0) k = last;                                         // u s was reached by rounding only
+  }
+  const bool fine = s > 0.0 && s < __builtin_inf();              // (false for NaN)
+  store_action(action, vocab, i, fine ? k : 0);
+  lp[i] = fine ? (float)((double)l[k] - (double)m - log(s)) : __builtin_nanf("");
+}
+
+// A workgroup of sixteen waves per row; a wave owns one contiguous sixteenth.  Pass 1: the maximum; pass 2: the waves' sums; then the one wave whose
+// part holds the border walks it, 64 lanes x 8 elements at a time.
+template <class T>
+__global__ __launch_bounds__(1024) void k_sample_rows(const T* logits, int64_t ld, int64_t vocab, const float* u, void* action, float* lp) {
+  __shared__ float wm[16];
+  __shared__ int64_t wi[16];
+  __shared__ double ws[16];
+  __shared__ int64_t wl[16];
+  constexpr int E = 8;
+  const int64_t i = blockIdx.x;
+  const T* row = logits + i * ld;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int64_t run = ((vocab + 15) / 16 + 64 * E - 1) / (64 * E) * (64 * E), from = min(vocab, w * run), to = min(vocab, from + run);
+  float m = NEG_INF;
+  int64_t at = vocab;
+  for (int64_t c = from + lane; c < to; c += 64) {
+    const float x = (float)row[c];
+    if (x > m) { m = x; at = c; }
+  }
+  const float M0 = wave_max(m);
+  int64_t a0 = m == M0 && m != NEG_INF ? at : vocab;
+#pragma unroll
+  for (int b = 32; b; b >>= 1) {
+    const int64_t o = (int64_t)(uint32_t)__shfl_xor((int)(uint32_t)a0, b) | (int64_t)__shfl_xor((int)(a0 >> 32), b) << 32;
+    a0 = min(a0, o);
+  }
+  if (lane == 0) { wm[w] = M0; wi[w] = a0; }
+  __syncthreads();
+  float M = wm[0];
+  int64_t best = wi[0];
+  for (int v = 1; v < 16; v++)
+    if (wm[v] > M) { M = wm[v]; best = wi[v]; }
+  double s = 0.0;
+  int64_t last = -1;
+  for (int64_t c = from + lane; c < to; c += 64) {
+    const double e = exp((double)(float)row[c] - (double)M);
+    s += e;
+    if (e > 0.0) last = c;
+  }
+  s = wave_sum(s);
+#pragma unroll
+  for (int b = 32; b; b >>= 1) {
+    const int64_t o = (int64_t)(uint32_t)__shfl_xor((int)(uint32_t)last, b) | (int64_t)__shfl_xor((int)(last >> 32), b) << 32;
+    last = max(last, o);
+  }
+  if (lane == 0) { ws[w] = s; wl[w] = last; }
+  __syncthreads();
+  double S = 0.0;
+  for (int v = 0; v < 16; v++) S += ws[v];
+  const bool fine = S > 0.0 && S < __builtin_inf();
+  if (!fine) {
+    if (threadIdx.x == 0) { store_action(action, vocab, i, 0); lp[i] = __builtin_nanf(""); }
+    return;
+  }
+  int64_t k = best;
+  if (u) {
+    const double target = (double)u[i] * S;
+    double before = 0.0;
+    int mine = -1;
+    int64_t end = 0;
+    for (int v = 0; v < 16; v++) {
+      if (wl[v] >= 0) { end = wl[v]; if (before + ws[v] > target) { mine = v; break; } }
+      before += ws[v];
+    }
+    k = end;                                                     // u s was reached by rounding only: the last element that has a share
+    if (mine >= 0) {
+      if (w != mine) return;
+      bool found = false;
+      for (int64_t c0 = from; c0 < to && !found; c0 += 64 * E) {
+        double e[E], sum = 0.0;
+#pragma unroll
+        for (int q = 0; q < E; q++) {
+          const int64_t c = c0 + lane * E + q;
+          e[q] = c < to ? exp((double)(float)row[c] - (double)M) : 0.0;
+          sum += e[q];
+        }
+        double upto = sum;                                       // inclusive over the lanes
+#pragma unroll
+        for (int b = 1; b < 64; b <<= 1) {
+          const double o = __hiloint2double(__shfl_up(__double2hiint(upto), b), __shfl_up(__double2loint(upto), b));
+          if (lane >= b) upto += o;
+        }
+        const unsigned long long hit = __ballot(before + upto > target && sum > 0.0);
+        if (hit) {
+          found = true;
+          if (lane == __ffsll((long long)hit) - 1) {
+            double r = before + (upto - sum);
+            int64_t pick = -1, some = -1;
+#pragma unroll
+            for (int q = 0; q < E; q++) {
+              r += e[q];
+              if (e[q] > 0.0) { some = c0 + lane * E + q; if (pick < 0 && r > target) pick = some; }
+            }
+            k = pick >= 0 ? pick : some;
+            store_action(action, vocab, i, k);
+            lp[i] = (float)((double)(float)row[k] - (double)M - log(S));
+          }
+        }
+        before += __hiloint2double(__shfl(__double2hiint(upto), 63), __shfl(__double2loint(upto), 63));
+      }
+      if (found) return;
+      if (lane) return;
+    } else if (threadIdx.x) return;
+  } else if (threadIdx.x) return;
+  store_action(action, vocab, i, k);
+  lp[i] = (float)((double)(float)row[k] - (double)M - log(S));
+}
+
+static int check_logits(int dtype, int64_t rows, int64_t vocab, int64_t ld) {
+  if (dtype != MG_DT_F32 && dtype != MG_DT_BF16 && dtype != MG_DT_F16) return fail(MG_ERR_INVALID, "logits must be f32, bf16 or f16");
+  if (rows < 0 || rows > 0x7fffffffll || vocab < 1 || vocab > 0x7fffffffll) return fail(MG_ERR_INVALID, "sizes must be 0 <= rows, 1 <= vocab, below 2^31");
+  if (ld < vocab) return fail(MG_ERR_INVALID, "the row stride is smaller than a row");
+  return MG_OK;
+}
+
+static int check_action(int t) { return t == MG_DT_U8 || t == MG_DT_I32 || t == MG_DT_I64 ? MG_OK : fail(MG_ERR_INVALID, "action must be u8, i32 or i64"); }
+
+static int small_rows(int64_t vocab) { return vocab < 32 ? 256 : 64; }            // rows per workgroup: at most 32 KB of LDS
+
+template <class F> static int by_type(int dtype, F f) {
+  return dtype == MG_DT_F32 ? f((const float*)nullptr) : dtype == MG_DT_BF16 ? f((const bf16*)nullptr) : f((const f16*)nullptr);
+}
+
+static size_t small_lds(int R, int64_t vocab) { return std::max<size_t>((size_t)R * (vocab | 1) * 4, 4 * sizeof(Terms)); }
+
+}  // namespace mgo
+
+using namespace mgo;
+
+extern "C" {
+
+int mg_op_policy_loss_workspace(int64_t rows, int64_t vocab, int64_t* bytes) {
+  const int rc = check_logits(MG_DT_F32, rows, vocab, vocab);
+  if (rc != MG_OK) return rc;
+  *bytes = (vocab <= SMALL_VOCAB ? (rows + small_rows(vocab) - 1) / small_rows(vocab) : rows) * (int64_t)sizeof(Terms);
+  return MG_OK;
+}
+
+int mg_op_policy_loss(int device, void* stream, int dtype, int64_t rows, int64_t vocab, const void* logits, int64_t ld, const void* action, int action_dtype, const float* old_lp,
+                      const float* adv, const float* ref_lp, const uint8_t* mask, double clip_lo, double clip_hi, double kl_coef, double ent_coef, float* out,
+                      void* save, void* ws, int64_t ws_bytes) {
+  int rc = check_logits(dtype, rows, vocab, ld);
+  if (rc == MG_OK) rc = check_action(action_dtype);
+  if (rc != MG_OK) return rc;
+  if (!out || (rows && (!logits || !action || !old_lp || !adv))) return fail(MG_ERR_INVALID, "logits, action, old_lp, adv and out must not be NULL");
+  int64_t need = 0;
+  mg_op_policy_loss_workspace(rows, vocab, &need);
+  if (ws_bytes < need || (need && (!ws || ((uintptr_t)ws & 15)))) return fail(MG_ERR_INVALID, "workspace: %lld bytes are needed", (long long)need);
+  DeviceGuard g(device);
+  if (g.rc != MG_OK) return g.rc;
+  hipStream_t st = (hipStream_t)stream;
+  LossArgs a = {logits, ld, action, action_dtype, old_lp, adv, ref_lp, mask, 1.0 - clip_lo, 1.0 + clip_hi, kl_coef, ent_coef, (Saved*)save, rows, vocab};
+  int64_t parts = 0;
+  if (rows && vocab <= SMALL_VOCAB) {
+    const int R = small_rows(vocab);
+    parts = (rows + R - 1) / R;
+    by_type(dtype, [&](auto* t) {
+      typedef std::remove_cv_t<std::remove_pointer_t<decltype(t)>> T;
+      k_loss_small<T><<<(unsigned)parts, R, small_lds(R, vocab), st>>>(a, (Terms*)ws, out);
+      return 0;
+    });
+    if (parts == 1) return launched("policy loss");
+  } else if (rows) {
+    parts = rows;
+    by_type(dtype, [&](auto* t) {
+      typedef std::remove_cv_t<std::remove_pointer_t<decltype(t)>> T;
+      k_loss_rows<T><<<(unsigned)rows, 256, 0, st>>>(a, (Terms*)ws);
+      return 0;
+    });
+  }
+  k_loss_out<<<1, 256, 0, st>>>(a, parts, (const Terms*)ws, out);
+  return launched("policy loss");
+}
+
+int mg_op_policy_loss_backward(int device, void* stream, int dtype, int64_t rows, int64_t vocab, const void* logits, int64_t ld, const void* action, int action_dtype,
+                               const uint8_t* mask, double ent_coef, const float* out, const void* save, const float* grad, void* dlogits) {
+  int rc = check_logits(dtype, rows, vocab, ld);
+  if (rc == MG_OK) rc = check_action(action_dtype);
+  if (rc != MG_OK || rows == 0) return rc;
+  if (!logits || !action || !out || !save || !grad || !dlogits) return fail(MG_ERR_INVALID, "no pointer but mask may be NULL");
+  DeviceGuard g(device);
+  if (g.rc != MG_OK) return g.rc;
+  hipStream_t st = (hipStream_t)stream;
+  GradArgs a = {logits, ld, action, action_dtype, mask, (const Saved*)save, out, grad, dlogits, (float)ent_coef, rows, vocab};
+  return by_type(dtype, [&](auto* t) {
+    typedef std::remove_cv_t<std::remove_pointer_t<decltype(t)>> T;
+    if (vocab <= SMALL_VOCAB) {
+      const int R = small_rows(vocab);
+      k_grad_small<T><<<(unsigned)((rows + R - 1) / R), R, small_lds(R, vocab), st>>>(a);
+    } else {
+      const int64_t runs = (vocab + GRAD_RUN - 1) / GRAD_RUN;
+      if (runs > 65535) return fail(MG_ERR_INVALID, "vocab above 2^30 is not supported");
+      k_grad_rows<T><<<dim3((unsigned)rows, (unsigned)runs), 256, 0, st>>>(a);
+    }
+    return launched("policy loss backward");
+  });
+}
+
+int mg_op_sample(int device, void* stream, int dtype, int64_t rows, int64_t vocab, const void* logits, int64_t ld, const float* u, void* action, float* lp) {
+  int rc = check_logits(dtype, rows, vocab, ld);
+  if (rc != MG_OK || rows == 0) return rc;
+  if (!logits || !action || !lp) return fail(MG_ERR_INVALID, "logits, action and lp must not be NULL");
+  DeviceGuard g(device);
+  if (g.rc != MG_OK) return g.rc;
+  hipStream_t st = (hipStream_t)stream;
+  return by_type(dtype, [&](auto* t) {
+    typedef std::remove_cv_t<std::remove_pointer_t<decltype(t)>> T;
+    if (vocab <= SMALL_VOCAB) {
+      const int R = small_rows(vocab);
+      k_sample_small<T><<<(unsigned)((rows + R - 1) / R), R, (size_t)R * (vocab | 1) * 4, st>>>((const T*)logits, ld, rows, (int)vocab, u, action, lp);
+    } else {
+      k_sample_rows<T><<<(unsigned)rows, 1024, 0, st>>>((const T*)logits, ld, vocab, u, action, lp);
+    }
+    return launched("sample");
+  });
+}
+
+}  // extern "C"

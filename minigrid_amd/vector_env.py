@@ -441,12 +441,70 @@ class MiniGridVecEnv(_VectorEnvBase):
             raise ValueError("final_obs=True reports terminal observations from step(), one launch at a time; "
                              "the fused entry points need autoreset_mode='same_step' without it (or 'next_step')")
 
-    def rollout(self, steps: int, action_seed: int = 0, fused: bool = False):
+    def rollout(self, steps: int, action_seed: int = 0, fused: bool = False, policy=None):
         """`steps` lockstep steps under a uniform-random policy generated on the device (the loop of
         minigrid/benchmark.py:36-43).  fused: up to `max_fused_steps` steps per kernel launch, the grids resident in
-        LDS; step j writes trajectory slot (steps-1-j) % traj_slots, so slot 0 is the last step."""
+        LDS; step j writes trajectory slot (steps-1-j) % traj_slots, so slot 0 is the last step.
+
+        policy: a callable that takes an observation as `step` returns it and gives (logits (num_envs, 7), value (num_envs,)) --
+        minigrid_amd.policy.ActorCritic, or any other.  The actions are then drawn from its logits (`sample_actions`; action_seed seeds the draws), one
+        launch per step, and the transitions come back as a minigrid_amd.policy.Trajectory.  Needs output="torch"; no gradient is recorded."""
+        if policy is not None:
+            return self._rollout_policy(int(steps), int(action_seed), bool(fused), policy)
         self._no_fused_with_final_obs()
         B.check(self._lib.mg_rollout(self._h, int(steps), int(action_seed), int(fused)), self._h)
+
+    def _rollout_policy(self, steps, action_seed, fused, policy):
+        if self.output != "torch":
+            raise ValueError("rollout(policy=...) needs an env made with output='torch'")
+        if fused:
+            raise ValueError("a policy is asked once per step: fused=True belongs to the device's own uniform policy")
+        if steps < 1:
+            raise ValueError("steps must be at least 1")
+        mode = self.metadata["autoreset_mode"]
+        if mode == "disabled":
+            raise ValueError("rollout(policy=...) needs an autoreset: autoreset_mode 'next_step' or 'same_step'")
+        self._no_fused_with_final_obs()
+        import torch
+
+        from .ops import sample_actions
+        from .policy import Trajectory
+        dev, n = torch.device("cuda", self.device), self.num_envs
+        if torch.cuda.current_stream(dev).cuda_stream != (self._stream_arg or 0):
+            raise ValueError("rollout(policy=...) runs on the stream that was current when the env was made")
+        with torch.no_grad(), torch.cuda.device(dev):
+            out, lay = self.torch_outputs(), self.record_layout()
+            # a step's scalars are one record per env: they are kept as they lie (the reward in front, see mg_step_scalars)
+            at, width = lay["reward"], lay["scalar_stride"]
+            now = out["record"][at:at + n * width].view(n, width)
+            rec = torch.empty((steps, n, width), dtype=torch.uint8, device=dev)
+            before = torch.empty_like(rec)
+            image = torch.empty((steps,) + tuple(out["image"].shape), dtype=out["image"].dtype, device=dev)
+            action = torch.empty((steps, n), dtype=torch.uint8, device=dev)
+            log_prob = torch.empty((steps, n), dtype=torch.float32, device=dev)
+            value = torch.empty((steps, n), dtype=torch.float32, device=dev)
+            u = torch.rand((steps, n), generator=torch.Generator(dev).manual_seed(action_seed), device=dev)
+            done = (out["terminated"] | out["truncated"]).bool()
+            obs = self._collect()[0]
+            for t in range(steps):
+                image[t].copy_(out["image"])
+                before[t].copy_(now)
+                logits, v = policy(obs)
+                if logits.shape != (n, 7) or v.shape != (n,):
+                    raise ValueError(f"policy must give logits {(n, 7)} and value {(n,)}, got {tuple(logits.shape)} and {tuple(v.shape)}")
+                a, lp = sample_actions(logits, u[t])
+                action[t].copy_(a)
+                log_prob[t].copy_(lp)
+                value[t].copy_(v)
+                B.check(self._lib.mg_step(self._h, C.c_void_p(action[t].data_ptr()), B.ACT_U8, 1), self._h)
+                rec[t].copy_(now)
+                obs = self._collect()[0]
+            last = policy(obs)[1].float().clone()
+        field = lambda r, name: r[:, :, lay[name] - at]
+        return Trajectory(image=image, direction=field(before, "direction"),
+                          mission_id=before.view(torch.int16)[:, :, (lay["mission_id"] - at) // 2], action=action, log_prob=log_prob, value=value,
+                          reward=rec.view(torch.float64)[:, :, 0], terminated=field(rec, "terminated"), truncated=field(rec, "truncated"), done=done,
+                          last_value=last, autoreset_mode=mode)
 
     def rollout_block(self, steps: int, action_seed: int = 0, slot0: Optional[int] = None):
         """ONE fused launch of `steps` <= max_fused_steps steps of the device policy; step j lands in trajectory slot slot0 - j
