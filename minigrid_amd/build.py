@@ -47,6 +47,7 @@ for _g in ("rooms", "sentence", "roomgrid", "light"):
 # the learning operators (include/minigrid_ops.h): no kernel of the environments sees them
 _OPS = ["ops/mg_ops.h", os.path.join("..", "..", "include", "minigrid_ops.h"), ABI_HEADER]
 UNITS.update({"ops/mg_linear.hip": _OPS + ["ops/mg_linear.h"], "ops/mg_policy.hip": _OPS, "ops/mg_advantages.hip": _OPS})
+UNITS.update({f"ops/mg_linear_{t}.hip": _OPS + ["ops/mg_linear.h", "ops/mg_linear_tu.inc"] for t in ("bf16", "f16", "f32")})
 # no packed 32-bit float instructions in them: ordinary float code would be turned into them
 UNIT_FLAGS = {u: ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"] for u in UNITS if u.startswith("ops/")}
 # the slowest units (minutes) first, so that the pool does not end on one of them

@@ -7,8 +7,11 @@
 //
 // An operand that is contiguous along s ("rows") lies in LDS as 128-byte rows of one tile row each; one that is contiguous along i / j ("cols") lies
 // there as one row per s and is turned by the transposing LDS read (16-bit types) or read element by element (f32).  Both are swizzled so that the
-// fragment reads of a wave spread over all banks.  Global loads go through registers: they may be unaligned, partial (guarded), or bytes that are
-// widened on the way.  The loads of tile t + 1 are in flight while tile t is multiplied (two LDS buffers, one barrier per tile).
+// fragment reads of a wave spread over all banks.  Global loads go through registers: rows may start at any address, and bytes are widened on the way.
+//
+// Two kernels.  k_product takes results at least as large as its tile and at least one tile deep, and then needs no bounds check at all: a tile that would
+// stick out is moved back inside (its first rows belong to a neighbour and are not stored), and a last piece of the summed axis is loaded as the last
+// whole one with what was summed already set to zero.  k_product_guarded checks every chunk and takes the rest.
 #pragma once
 #include "mg_ops.h"
 
@@ -111,15 +114,15 @@ __device__ __forceinline__ float activate_grad(int act, float z) {
 }
 
 // ---- global loads ----
-// N consecutive elements of a memory row as T, element e valid where at + e < end; VEC: 16-byte aligned and never partial
-template <class T, class S, bool VEC>
+// N consecutive elements of a memory row as T, element e valid where at + e < end
+template <class T, class S>
 __device__ __forceinline__ typename Chunk<T>::V load_chunk(const S* row, int64_t at, int64_t end, bool inside) {
   constexpr int N = Chunk<T>::N;
   typename Chunk<T>::V v = {};
   if (!inside || at >= end) return v;
   if constexpr (sizeof(S) == sizeof(T)) {
-    if (VEC || at + N <= end) {
-      __builtin_memcpy(&v, VEC ? __builtin_assume_aligned(row + at, 16) : (const void*)(row + at), 16);
+    if (at + N <= end) {
+      __builtin_memcpy(&v, row + at, 16);
       return v;
     }
   } else if (at + N <= end) {
@@ -136,12 +139,10 @@ __device__ __forceinline__ typename Chunk<T>::V load_chunk(const S* row, int64_t
 }
 
 // One operand's tile: EXT rows of the result x 128 / sizeof(T) summed elements = EXT x 128 bytes of LDS.
-template <class T, class S, bool COLS, bool VEC, int EXT, int THREADS>
-struct Tile {
+template <class T, bool COLS, int EXT>
+struct Lds {
   typedef typename Chunk<T>::V V;
-  static constexpr int N = Chunk<T>::N, BK = 8 * N, BYTES = EXT * 128, PER = EXT * 8 / THREADS;
-  static_assert(EXT * 8 % THREADS == 0, "whole chunks per thread");
-  V hold[PER];
+  static constexpr int N = Chunk<T>::N, BK = 8 * N, BYTES = EXT * 128, CPR = COLS ? EXT / N : 8;       // CPR: chunks per row of memory
 
   // LDS byte address of the chunk (row i, s = c * N ..) / (s, i = c * N ..)
   static __device__ __forceinline__ int addr_rows(int i, int c) { return i * 128 + ((c ^ (i & 7)) << 4); }
@@ -151,30 +152,9 @@ struct Tile {
   }
   static __device__ __forceinline__ int addr_cols(int s, int byte) { return s * (EXT * (int)sizeof(T)) + (byte ^ swz(s)); }
 
-  __device__ __forceinline__ void load(const Operand& o, int i0, int64_t s0, int64_t send) {
-    const S* p = (const S*)o.p;
-#pragma unroll
-    for (int q = 0; q < PER; q++) {
-      const int u = q * THREADS + (int)threadIdx.x;
-      if constexpr (!COLS) {
-        const int i = u >> 3, c = u & 7;
-        hold[q] = load_chunk<T, S, VEC>(p + (int64_t)(i0 + i) * o.ld, s0 + c * N, send, i0 + i < o.extent);
-      } else {
-        constexpr int CPR = EXT / N;                      // chunks per row of memory
-        const int s = u / CPR, c = u % CPR;
-        hold[q] = load_chunk<T, S, VEC>(p + (s0 + s) * o.ld, (int64_t)i0 + c * N, o.extent, s0 + s < send);
-      }
-    }
-  }
-  __device__ __forceinline__ void store(char* lds) const {
-#pragma unroll
-    for (int q = 0; q < PER; q++) {
-      const int u = q * THREADS + (int)threadIdx.x;
-      int a;
-      if constexpr (!COLS) a = addr_rows(u >> 3, u & 7);
-      else { constexpr int CPR = EXT / N; a = addr_cols(u / CPR, (u % CPR) * 16); }
-      *(V*)(lds + a) = hold[q];
-    }
+  // chunk u of the tile, in the order of memory
+  static __device__ __forceinline__ void put(char* lds, int u, V v) {
+    *(V*)(lds + (COLS ? addr_cols(u / CPR, (u % CPR) * 16) : addr_rows(u / CPR, u % CPR))) = v;
   }
   // what lane l feeds in step c of the tile: row i0 + l % 32, the N summed elements (2 c + l / 32) * N ..
   static __device__ __forceinline__ V frag(const char* lds, int i0, int c) {
@@ -197,6 +177,74 @@ struct Tile {
   }
 };
 
+// A thread's chunks of a tile on their way from memory to LDS, every one checked
+template <class T, class S, bool COLS, int EXT, int THREADS>
+struct GuardedLoader {
+  typedef Lds<T, COLS, EXT> L;
+  static constexpr int PER = EXT * 8 / THREADS;
+  static_assert(EXT * 8 % THREADS == 0, "whole chunks per thread");
+  typename L::V hold[PER];
+  __device__ __forceinline__ void load(const Operand& o, int i0, int64_t s0, int64_t send) {
+    const S* p = (const S*)o.p;
+#pragma unroll
+    for (int q = 0; q < PER; q++) {
+      const int u = q * THREADS + (int)threadIdx.x, r = u / L::CPR, c = (u % L::CPR) * L::N;
+      if constexpr (!COLS) hold[q] = load_chunk<T, S>(p + (int64_t)(i0 + r) * o.ld, s0 + c, send, i0 + r < o.extent);
+      else hold[q] = load_chunk<T, S>(p + (s0 + r) * o.ld, (int64_t)i0 + c, o.extent, s0 + r < send);
+    }
+  }
+  __device__ __forceinline__ void store(char* lds) const {
+#pragma unroll
+    for (int q = 0; q < PER; q++) L::put(lds, q * THREADS + (int)threadIdx.x, hold[q]);
+  }
+};
+
+// The same without checks: the tile lies inside the operand.  One 32-bit offset per thread (the host has checked that a tile spans less than 2 GiB); what
+// differs between a thread's chunks and between tiles is uniform.
+template <class T, class S, bool COLS, int EXT, int THREADS>
+struct Loader {
+  typedef Lds<T, COLS, EXT> L;
+  static constexpr int PER = EXT * 8 / THREADS, N = L::N, BK = L::BK;
+  static_assert(EXT * 8 % THREADS == 0 && THREADS % L::CPR == 0, "whole chunks and rows per pass of the threads");
+  typedef uint8_t Bytes __attribute__((ext_vector_type(N)));
+  typedef std::conditional_t<sizeof(S) == 1, Bytes, typename L::V> Raw;
+  Raw hold[PER];
+  const char* base;            // of the tile that is loaded next
+  int64_t pass, step;          // bytes between a thread's chunks, and between tiles
+  uint32_t off;
+  __device__ __forceinline__ void start(const Operand& o, int i0, int64_t s0) {
+    const int r = (int)threadIdx.x / L::CPR, c = (int)threadIdx.x % L::CPR;
+    off = (uint32_t)(r * (int)(o.ld * sizeof(S)) + c * (int)(N * sizeof(S)));
+    pass = (int64_t)(THREADS / L::CPR) * o.ld * sizeof(S);
+    step = (COLS ? BK * o.ld : BK) * (int64_t)sizeof(S);
+    base = (const char*)o.p + (COLS ? s0 * o.ld + i0 : (int64_t)i0 * o.ld + s0) * (int64_t)sizeof(S);
+  }
+  __device__ __forceinline__ void back(const Operand& o, int64_t by) { base -= (COLS ? by * o.ld : by) * (int64_t)sizeof(S); }
+  __device__ __forceinline__ void load() {
+#pragma unroll
+    for (int q = 0; q < PER; q++) __builtin_memcpy(&hold[q], base + q * pass + off, sizeof(Raw));
+    base += step;
+  }
+  // done: so many leading elements of the summed axis were summed before
+  __device__ __forceinline__ void store(char* lds, int done) const {
+#pragma unroll
+    for (int q = 0; q < PER; q++) {
+      const int u = q * THREADS + (int)threadIdx.x;
+      typename L::V v;
+      if constexpr (sizeof(S) == 1) {
+#pragma unroll
+        for (int e = 0; e < N; e++) v[e] = (T)(float)hold[q][e];
+      } else v = hold[q];
+      if (done) {
+        const int at = COLS ? u / L::CPR : (u % L::CPR) * N;
+#pragma unroll
+        for (int e = 0; e < N; e++) v[e] = at + (COLS ? 0 : e) < done ? (T)0.0f : v[e];
+      }
+      L::put(lds, u, v);
+    }
+  }
+};
+
 __device__ __forceinline__ f32x16 mma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x16 mma(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x16 mma(f32x4 a, f32x4 b, f32x16 c) {   // both operands deal the summed index alike, so its order does not matter
@@ -205,10 +253,10 @@ __device__ __forceinline__ f32x16 mma(f32x4 a, f32x4 b, f32x16 c) {   // both op
   return c;
 }
 
-// W consecutive elements (i, j ..) of the result, `count` of them inside; the sums come in 32 bits and each result is rounded to T once.  WIDE: all of
+// W consecutive elements (i, j ..) of the result, those from `skip` up to `count` to be stored; the sums come in 32 bits and each result is rounded to T once.  WIDE: all of
 // them inside and every row 16-byte aligned.
 template <class T, int W, bool WIDE>
-__device__ __forceinline__ void finish(const Epilogue& e, int64_t i, int64_t j, int64_t n, int count, float (&v)[W]) {
+__device__ __forceinline__ void finish(const Epilogue& e, int64_t i, int64_t j, int64_t n, int skip, int count, float (&v)[W]) {
   T t[W];
   if (e.b) {
 #pragma unroll
@@ -223,7 +271,7 @@ __device__ __forceinline__ void finish(const Epilogue& e, int64_t i, int64_t j, 
     else
 #pragma unroll
       for (int u = 0; u < W; u++)
-        if (u < count) z[u] = t[u];
+        if (u >= skip && u < count) z[u] = t[u];
   }
   switch (e.act) {
 #define MG_ACT(A) case A: _Pragma("unroll") for (int u = 0; u < W; u++) v[u] = activate(A, v[u]); break;
@@ -250,27 +298,87 @@ __device__ __forceinline__ void finish(const Epilogue& e, int64_t i, int64_t j, 
   else
 #pragma unroll
     for (int u = 0; u < W; u++)
-      if (u < count) c[u] = t[u];
+      if (u >= skip && u < count) c[u] = t[u];
 }
 
-// grid: (tiles, splits); WI x WJ waves of (BI / WI) x (BJ / WJ) each
-template <class T, class SA, class SB, bool ACOLS, bool BCOLS, bool VEC, int BI, int BJ, int WI, int WJ>
-__global__ __launch_bounds__(WI * WJ * 64) void k_product(Operand A, Operand B, int64_t depth, int32_t depth_tiles_per_split, Epilogue ep) {
-  constexpr int THREADS = WI * WJ * 64, MI = BI / WI / 32, MJ = BJ / WJ / 32;
-  typedef Tile<T, SA, ACOLS, VEC, BI, THREADS> TA;
-  typedef Tile<T, SB, BCOLS, VEC, BJ, THREADS> TB;
-  constexpr int BK = TA::BK;
-  __shared__ __attribute__((aligned(16))) char lds[2 * (TA::BYTES + TB::BYTES)];
+// Workgroups go to the eight XCDs in turn: each XCD takes one contiguous run of tiles, ordered in bands of eight tile rows with the row running fastest, so
+// that what is multiplied at the same time on an XCD is a block of tiles that shares rows of both operands in its L2.
+struct TileAt { int i, j; };
+__device__ __forceinline__ TileAt tile_at(int ti, int tj) {
+  const int tiles = gridDim.x, x = blockIdx.x & 7, run = tiles >> 3, more = tiles & 7;
+  const int t = x * run + min(x, more) + ((int)blockIdx.x >> 3);
+  const int band = t / (8 * tj), in = t - band * 8 * tj, high = min(8, ti - band * 8);
+  return {band * 8 + in % high, in / high};
+}
 
-  // workgroups go to the eight XCDs in turn: each XCD takes one contiguous run of tiles (j fastest), so that what shares rows of A shares an L2
-  const int tj = (B.extent + BJ - 1) / BJ, tiles = gridDim.x;
-  int t = blockIdx.x;
-  {
-    const int x = t & 7, run = tiles >> 3, more = tiles & 7;
-    t = x * run + min(x, more) + (t >> 3);
+// Lane l holds column l % 32 and rows 8 (q / 4) + 4 (l / 32) + q % 4 of a 32 x 32 block.  The sums pass through LDS, 32 rows of a wave at a time, so
+// that a lane ends with eight neighbours of one row: whole 16-byte accesses, whole lines.  (Row stride + 8: the two halves of a wave write disjoint banks.)
+// Rows below iown and columns below jown belong to a neighbour.
+template <class T, int MI, int MJ>
+__device__ __forceinline__ void store_tile(const Epilogue& ep, f32x16 (&acc)[MI][MJ], float* stage, int64_t i0, int64_t iown, int64_t iend, int64_t j0, int64_t jown, int64_t jend) {
+  constexpr int W = 8, STRIDE = MJ * 32 + 8, LPR = MJ * 32 / W, RPP = 64 / LPR;
+  const int l = threadIdx.x & 63;
+  const int64_t rows = iend, n = jend;
+#pragma unroll
+  for (int a = 0; a < MI; a++) {
+#pragma unroll
+    for (int b = 0; b < MJ; b++)
+#pragma unroll
+      for (int q = 0; q < 16; q++) stage[(8 * (q >> 2) + 4 * (l >> 5) + (q & 3)) * STRIDE + b * 32 + (l & 31)] = acc[a][b][q];
+    __builtin_amdgcn_wave_barrier();                             // (a wave's LDS operations happen in order)
+#pragma unroll 1
+    for (int p = 0; p < 32; p += RPP) {
+      const int row = p + l / LPR, col = (l % LPR) * W;
+      const int64_t i = i0 + a * 32 + row, j = j0 + col;
+      float v[W];
+      __builtin_memcpy(v, __builtin_assume_aligned(stage + row * STRIDE + col, 16), sizeof v);
+      const int count = (int)min((int64_t)W, jend - j), skip = (int)max((int64_t)0, jown - j);
+      if (i >= iown && i < iend && count > 0 && skip < W) {
+        if (ep.part) {
+          float* d = ep.part + ((int64_t)blockIdx.y * rows + i) * n + j;
+          if (ep.wide) __builtin_memcpy(__builtin_assume_aligned(d, 16), v, sizeof v);
+          else
+#pragma unroll
+            for (int u = 0; u < W; u++)
+              if (u >= skip && u < count) d[u] = v[u];
+        } else if (ep.wide) finish<T, W, true>(ep, i, j, n, 0, W, v);
+        else finish<T, W, false>(ep, i, j, n, skip, count, v);
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
   }
-  const int i0 = (t / tj) * BI, j0 = (t % tj) * BJ;
-  const int64_t s_begin = (int64_t)blockIdx.y * depth_tiles_per_split * BK, s_end = min(depth, s_begin + (int64_t)depth_tiles_per_split * BK);
+}
+
+template <class LA, class LB, int MI, int MJ>
+__device__ __forceinline__ void multiply(const char* la, const char* lb, int wi, int wj, int c, f32x16 (&acc)[MI][MJ]) {
+  typename LA::V fa[MI];
+  typename LB::V fb[MJ];
+#pragma unroll
+  for (int a = 0; a < MI; a++) fa[a] = LA::frag(la, wi + a * 32, c);
+#pragma unroll
+  for (int b = 0; b < MJ; b++) fb[b] = LB::frag(lb, wj + b * 32, c);
+#pragma unroll
+  for (int a = 0; a < MI; a++)
+#pragma unroll
+    for (int b = 0; b < MJ; b++) acc[a][b] = mma(fa[a], fb[b], acc[a][b]);
+}
+
+// grid: (tiles, splits); WI x WJ waves of (BI / WI) x (BJ / WJ) each; A.extent >= BI, B.extent >= BJ, depth >= BK
+template <class T, class SA, class SB, bool ACOLS, bool BCOLS, int BI, int BJ, int WI, int WJ>
+__global__ __launch_bounds__(WI * WJ * 64) void k_product(Operand A, Operand B, int64_t depth, int32_t tiles_per_split, Epilogue ep) {
+  constexpr int THREADS = WI * WJ * 64, MI = BI / WI / 32, MJ = BJ / WJ / 32;
+  typedef Loader<T, SA, ACOLS, BI, THREADS> TA;
+  typedef Loader<T, SB, BCOLS, BJ, THREADS> TB;
+  typedef typename TA::L LA;
+  typedef typename TB::L LB;
+  constexpr int BK = LA::BK, BUF = LA::BYTES + LB::BYTES;
+  __shared__ __attribute__((aligned(16))) char lds[2 * BUF];
+  const TileAt at = tile_at((A.extent + BI - 1) / BI, (B.extent + BJ - 1) / BJ);
+  const int i0 = min(at.i * BI, A.extent - BI), j0 = min(at.j * BJ, B.extent - BJ);
+  const int64_t first = (int64_t)blockIdx.y * tiles_per_split, deep = (depth + BK - 1) / BK;
+  const int tiles = (int)(min(deep, first + tiles_per_split) - first);
+  // (the last tile of the axis, if it is not whole, starts `over` earlier)
+  const int over = first + tiles == deep ? (int)(deep * BK - depth) : 0;
   const int wave = threadIdx.x >> 6, wi = (wave / WJ) * (BI / WI), wj = (wave % WJ) * (BJ / WJ);
 
   f32x16 acc[MI][MJ];
@@ -281,12 +389,66 @@ __global__ __launch_bounds__(WI * WJ * 64) void k_product(Operand A, Operand B, 
 
   TA ta;
   TB tb;
+  ta.start(A, i0, first * BK);
+  tb.start(B, j0, first * BK);
+  auto fetch = [&](int t) {
+    if (over && t == tiles - 1) { ta.back(A, over); tb.back(B, over); }
+    ta.load();
+    tb.load();
+  };
+  auto put = [&](int t) {
+    char* p = lds + (t & 1) * BUF;
+    const int done = t == tiles - 1 ? over : 0;
+    ta.store(p, done);
+    tb.store(p + LA::BYTES, done);
+  };
+  fetch(0);
+  put(0);
+  if (tiles > 1) fetch(1);
+  __syncthreads();
+  // while tile t is multiplied, tile t + 1 goes from registers to the other half of LDS and tile t + 2 is on its way from memory
+  for (int t = 0; t < tiles; t++) {
+    const char* la = lds + (t & 1) * BUF;
+    const char* lb = la + LA::BYTES;
+    multiply<LA, LB>(la, lb, wi, wj, 0, acc);
+    multiply<LA, LB>(la, lb, wi, wj, 1, acc);
+    if (t + 1 < tiles) put(t + 1);
+    if (t + 2 < tiles) fetch(t + 2);
+    multiply<LA, LB>(la, lb, wi, wj, 2, acc);
+    multiply<LA, LB>(la, lb, wi, wj, 3, acc);
+    __syncthreads();
+  }
+  static_assert(WI * WJ * 32 * (MJ * 32 + 8) * 4 <= (int)sizeof lds, "staging fits");
+  float* stage = (float*)lds + wave * 32 * (MJ * 32 + 8);
+  store_tile<T, MI, MJ>(ep, acc, stage, i0 + wi, at.i * (int64_t)BI, A.extent, j0 + wj, at.j * (int64_t)BJ, B.extent);
+}
+
+template <class T, class SA, class SB, bool ACOLS, bool BCOLS, int BI, int BJ, int WI, int WJ>
+__global__ __launch_bounds__(WI * WJ * 64) void k_product_guarded(Operand A, Operand B, int64_t depth, int32_t tiles_per_split, Epilogue ep) {
+  constexpr int THREADS = WI * WJ * 64, MI = BI / WI / 32, MJ = BJ / WJ / 32;
+  typedef GuardedLoader<T, SA, ACOLS, BI, THREADS> TA;
+  typedef GuardedLoader<T, SB, BCOLS, BJ, THREADS> TB;
+  typedef typename TA::L LA;
+  typedef typename TB::L LB;
+  constexpr int BK = LA::BK, BUF = LA::BYTES + LB::BYTES;
+  __shared__ __attribute__((aligned(16))) char lds[2 * BUF];
+  const TileAt at = tile_at((A.extent + BI - 1) / BI, (B.extent + BJ - 1) / BJ);
+  const int i0 = at.i * BI, j0 = at.j * BJ;
+  const int64_t s_begin = (int64_t)blockIdx.y * tiles_per_split * BK, s_end = min(depth, s_begin + (int64_t)tiles_per_split * BK);
+  const int wave = threadIdx.x >> 6, wi = (wave / WJ) * (BI / WI), wj = (wave % WJ) * (BJ / WJ);
+  f32x16 acc[MI][MJ];
+#pragma unroll
+  for (int a = 0; a < MI; a++)
+#pragma unroll
+    for (int b = 0; b < MJ; b++) acc[a][b] = (f32x16)(0.0f);
+  TA ta;
+  TB tb;
   ta.load(A, i0, s_begin, s_end);
   tb.load(B, j0, s_begin, s_end);
   int cur = 0;
   for (int64_t s = s_begin; s < s_end; s += BK) {
-    char* la = lds + cur * (TA::BYTES + TB::BYTES);
-    char* lb = la + TA::BYTES;
+    char* la = lds + cur * BUF;
+    char* lb = la + LA::BYTES;
     ta.store(la);
     tb.store(lb);
     if (s + BK < s_end) {
@@ -295,67 +457,114 @@ __global__ __launch_bounds__(WI * WJ * 64) void k_product(Operand A, Operand B, 
     }
     __syncthreads();
 #pragma unroll
-    for (int c = 0; c < 4; c++) {
-      typename TA::V fa[MI];
-      typename TB::V fb[MJ];
-#pragma unroll
-      for (int a = 0; a < MI; a++) fa[a] = TA::frag(la, wi + a * 32, c);
-#pragma unroll
-      for (int b = 0; b < MJ; b++) fb[b] = TB::frag(lb, wj + b * 32, c);
-#pragma unroll
-      for (int a = 0; a < MI; a++)
-#pragma unroll
-        for (int b = 0; b < MJ; b++) acc[a][b] = mma(fa[a], fb[b], acc[a][b]);
-    }
+    for (int c = 0; c < 4; c++) multiply<LA, LB>(la, lb, wi, wj, c, acc);
     cur ^= 1;
   }
-
-  // Lane l holds column l % 32 and rows 8 (q / 4) + 4 (l / 32) + q % 4 of a 32 x 32 block.  The sums pass through LDS, 32 rows of a wave at a time, so
-  // that a lane ends with eight neighbours of one row: whole 16-byte accesses, whole lines.  (Row stride + 8: the two halves of a wave write disjoint banks.)
-  constexpr int W = 8, COLS = BJ / WJ, STRIDE = COLS + 8, LPR = COLS / W, RPP = 64 / LPR;
-  static_assert(WI * WJ * 32 * STRIDE * 4 <= (int)sizeof lds, "staging fits");
-  const int l = threadIdx.x & 63;
-  float* stage = (float*)lds + wave * 32 * STRIDE;
   __syncthreads();
+  static_assert(WI * WJ * 32 * (MJ * 32 + 8) * 4 <= (int)sizeof lds, "staging fits");
+  float* stage = (float*)lds + wave * 32 * (MJ * 32 + 8);
+  store_tile<T, MI, MJ>(ep, acc, stage, i0 + wi, 0, A.extent, j0 + wj, 0, B.extent);
+}
+
+// Few rows (a step of a handful of environments): a wave per result column, its lanes along k in chunks of 16 bytes of the weight, one sum per row and lane,
+// joined over the lanes at the end.  Bound by the weight's bytes where it is large, by one trip to memory and back where it is small.
+template <class T, class S, int ROWS>
+__global__ __launch_bounds__(256) void k_few_rows(int rows, int64_t k, int64_t n, const S* x, int64_t ldx, const T* w, int64_t ldw, Epilogue ep) {
+  constexpr int N = Chunk<T>::N;
+  const int lane = threadIdx.x & 63;
+  const int64_t j = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (j >= n) return;
+  const T* wj = w + j * ldw;
+  float s[ROWS];
 #pragma unroll
-  for (int a = 0; a < MI; a++) {
+  for (int i = 0; i < ROWS; i++) s[i] = 0.0f;
+  for (int64_t c = (int64_t)lane * N; c < k; c += 64 * N) {
+    const auto b = load_chunk<T, T>(wj, c, k, true);
 #pragma unroll
-    for (int b = 0; b < MJ; b++)
+    for (int i = 0; i < ROWS; i++) {
+      if (i < rows) {
+        const auto a = load_chunk<T, S>(x + i * ldx, c, k, true);
 #pragma unroll
-      for (int q = 0; q < 16; q++) stage[(8 * (q >> 2) + 4 * (l >> 5) + (q & 3)) * STRIDE + b * 32 + (l & 31)] = acc[a][b][q];
-    __syncthreads();
-#pragma unroll 1
-    for (int p = 0; p < 32; p += RPP) {
-      const int row = p + l / LPR, col = (l % LPR) * W;
-      const int64_t i = i0 + wi + a * 32 + row, j = j0 + wj + col;
-      float v[W];
-      __builtin_memcpy(v, __builtin_assume_aligned(stage + row * STRIDE + col, 16), sizeof v);
-      const int count = (int)min((int64_t)W, (int64_t)B.extent - j);
-      if (i < A.extent && count > 0) {
-        if (ep.part) {
-          float* d = ep.part + ((int64_t)blockIdx.y * A.extent + i) * B.extent + j;
-          if (ep.wide) __builtin_memcpy(__builtin_assume_aligned(d, 16), v, sizeof v);
-          else
-#pragma unroll
-            for (int u = 0; u < W; u++)
-              if (u < count) d[u] = v[u];
-        } else if (ep.wide) finish<T, W, true>(ep, i, j, B.extent, W, v);
-        else finish<T, W, false>(ep, i, j, B.extent, count, v);
+        for (int e = 0; e < N; e++) s[i] = __builtin_fmaf((float)a[e], (float)b[e], s[i]);
       }
+    }
+  }
+  float mine = 0.0f;
+#pragma unroll
+  for (int i = 0; i < ROWS; i++) {
+#pragma unroll
+    for (int m = 32; m; m >>= 1) s[i] += __shfl_xor(s[i], m);
+    mine = lane == i ? s[i] : mine;
+  }
+  if (lane < rows) {
+    float v[1] = {mine};
+    finish<T, 1, false>(ep, lane, j, n, 0, 1, v);
+  }
+}
+
+// The splits' sums, added in an order that the sizes fix, and the epilogue.  A workgroup takes 256 neighbouring results: a wave reads a quarter of the splits,
+// four results a lane, and the four sums of a result meet in LDS.
+template <class T>
+__global__ __launch_bounds__(256) void k_join(int64_t total, int64_t n, int splits, Epilogue ep) {
+  __shared__ float sum[4][256];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  for (int64_t u0 = (int64_t)blockIdx.x * 256; u0 < total; u0 += (int64_t)gridDim.x * 256) {
+    const int64_t u = u0 + lane * 4;
+    f32x4 s = (f32x4)(0.0f);
+    if (u + 4 <= total) {
+#pragma unroll 4
+      for (int q = w; q < splits; q += 4) {
+        f32x4 v;
+        __builtin_memcpy(&v, ep.part + (int64_t)q * total + u, 16);
+        s += v;
+      }
+    } else {
+      for (int q = w; q < splits; q += 4)
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          if (u + e < total) s[e] += ep.part[(int64_t)q * total + u + e];
+    }
+    *(f32x4*)&sum[w][lane * 4] = s;
+    __syncthreads();
+    const int64_t at = u0 + threadIdx.x;
+    if (at < total) {
+      float v[1] = {(sum[0][threadIdx.x] + sum[1][threadIdx.x]) + (sum[2][threadIdx.x] + sum[3][threadIdx.x])};
+      finish<T, 1, false>(ep, at / n, at % n, n, 0, 1, v);
     }
     __syncthreads();
   }
 }
 
-// the splits' sums, added in their order, and the epilogue
-template <class T>
-__global__ __launch_bounds__(256) void k_join(int64_t rows, int64_t n, int splits, Epilogue ep) {
-  const int64_t total = rows * n;
-  for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < total; u += (int64_t)gridDim.x * 256) {
-    float v[1] = {0.0f};
-    for (int s = 0; s < splits; s++) v[0] += ep.part[(int64_t)s * total + u];
-    finish<T, 1, false>(ep, u / n, u % n, n, 1, v);
-  }
+// ---- what mg_linear.hip asks of the translation unit of a type ----
+enum { TILE_GUARDED_32_128, TILE_GUARDED_128_32, TILE_GUARDED_128_128, TILE_64, TILE_128, TILE_256, TILES };
+enum { FORM_FORWARD, FORM_DX, FORM_DW };          // A rows B rows, A rows B cols, A cols B cols
+struct Plan {
+  int tile, splits, per;       // how many ways the summed axis is split, tiles of that axis per split
+  int64_t part_bytes;
+};
+constexpr int TILE_I[TILES] = {32, 128, 128, 64, 128, 256}, TILE_J[TILES] = {128, 32, 128, 64, 128, 256};
+constexpr int FEW_ROWS = 8;
+template <class T> struct Linear {
+  static void product(hipStream_t st, int form, bool bytes, const Plan& p, const Operand& A, const Operand& B, int64_t depth, const Epilogue& ep);
+  static void few_rows(hipStream_t st, bool bytes, int rows, int64_t k, int64_t n, const void* x, int64_t ldx, const void* w, int64_t ldw, const Epilogue& ep);
+  static void join(hipStream_t st, int64_t rows, int64_t n, int splits, const Epilogue& ep);
+  static void dz(hipStream_t st, int act, int64_t rows, int64_t n, const void* dy, int64_t lddy, const void* z, void* dz, void* db, float* part);
+};
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// dz = dy act'(z) and the column sums of dz: a workgroup takes `lanes` chunks of eight columns and every 256 / lanes-th row of a run
+struct DzPlan { int lanes_log2; int64_t strips, run, runs; };
+inline DzPlan dz_plan(int64_t rows, int64_t n) {
+  DzPlan p;
+  const int64_t chunks = ceil_div(n, 8);
+  p.lanes_log2 = 0;
+  while (p.lanes_log2 < 6 && (1 << p.lanes_log2) < chunks) p.lanes_log2++;
+  p.strips = ceil_div(chunks, 1 << p.lanes_log2);
+  // about four workgroups a CU, each with at least four rows a thread
+  const int64_t runs = std::max<int64_t>(1, 1024 / p.strips), least = 4 * (256 >> p.lanes_log2);
+  p.run = std::max<int64_t>(least, ceil_div(std::max<int64_t>(rows, 1), runs));
+  p.runs = ceil_div(std::max<int64_t>(rows, 1), p.run);
+  return p;
 }
 
 }  // namespace mgo
