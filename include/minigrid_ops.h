@@ -1,6 +1,7 @@
 /*
  * minigrid_ops.h — C ABI of the learning operators of libminigrid_hip.so: what turns the batched environments' observations into actions and their
- * trajectories into a gradient.  minigrid_amd/ops.py is the binding (torch tensors, autograd).
+ * trajectories into a gradient.  minigrid_amd/csrc/ops/mg_torch.cpp and minigrid_amd/ops.py are
+ * the binding (torch tensors, autograd).
  *
  * Conventions
  *   - plain C types only; every function returns MG_OK (0) or a negative mg_status (minigrid_hip.h); mg_ops_last_error() has the text of the calling
@@ -48,7 +49,7 @@ MG_API int mg_op_linear_dw(int device, void* stream, int dtype, int x_dtype, int
  * With lp = log softmax(logits)[action], q = exp(lp - old_lp), H = the entropy of softmax(logits), the loss is the mean over the counted rows of
  *     -min(q adv, clamp(q, 1 - clip_lo, 1 + clip_hi) adv) + kl_coef (exp(ref_lp - lp) - (ref_lp - lp) - 1) - ent_coef H.
  * out (6 f32): loss, mean policy term, mean KL term, mean entropy, share of clipped rows, number of counted rows.  No counted row: all 0.
- * save (rows x 16 bytes) and out are what the backward call needs; NULL save = no backward pass will follow.  Rows that do not count are not read.
+ * save ((rows + 1) x 16 bytes) is what the backward call needs; NULL = no backward pass will follow.  Rows that do not count are not read.
  * A counted row's action outside 0..vocab-1 makes the loss and the row's gradient NaN. */
 MG_API int mg_op_policy_loss_workspace(int64_t rows, int64_t vocab, int64_t* bytes);
 MG_API int mg_op_policy_loss(int device, void* stream, int dtype, int64_t rows, int64_t vocab, const void* logits, int64_t ld, const void* action, int action_dtype,
@@ -56,12 +57,14 @@ MG_API int mg_op_policy_loss(int device, void* stream, int dtype, int64_t rows, 
                              double ent_coef, float* out, void* save, void* ws, int64_t ws_bytes);
 /* dlogits (rows, vocab, contiguous) = grad[0] * d loss / d logits; rows that do not count get 0 */
 MG_API int mg_op_policy_loss_backward(int device, void* stream, int dtype, int64_t rows, int64_t vocab, const void* logits, int64_t ld, const void* action, int action_dtype,
-                                      const uint8_t* mask, double ent_coef, const float* out, const void* save, const float* grad, void* dlogits);
+                                      const uint8_t* mask, double ent_coef, const void* save, const float* grad, void* dlogits);
 
 /* ---- one draw per row: action = the lowest k with sum_{j<=k} e^{l_j} > u sum_j e^{l_j}, sums in 64 bits; u NULL: the lowest index of the largest logit ----
  * u (rows, f32 in [0, 1)); action: u8 where vocab <= 256, else i32; lp (rows, f32) = log softmax(logits)[action].  A row without a finite largest logit
  * gives action 0 and lp NaN. */
-MG_API int mg_op_sample(int device, void* stream, int dtype, int64_t rows, int64_t vocab, const void* logits, int64_t ld, const float* u, void* action, float* lp);
+MG_API int mg_op_sample_workspace(int64_t rows, int64_t vocab, int64_t* bytes);
+MG_API int mg_op_sample(int device, void* stream, int dtype, int64_t rows, int64_t vocab, const void* logits, int64_t ld, const float* u, void* action, float* lp,
+                        void* ws, int64_t ws_bytes);
 
 /* ---- generalised advantages of a rollout of `steps` x `envs` ----
  * reward (f64 or f32), value, terminated, truncated: element (t, e) at t * s?[0] + e * s?[1] elements; last_value (envs); done0 (envs, u8) or NULL: whether

@@ -22,6 +22,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libminigrid_hip.so")
 OBJDIR = os.path.join(CSRC, ".obj")
+TORCH_OPS = os.path.join(HERE, "_torch_ops.so")          # the learning operators' torch binding (csrc/ops/mg_torch.cpp)
 ABI_HEADER = os.path.join("..", "..", "include", "minigrid_hip.h")
 
 _COMMON = ["mg_device.h", "mg_rng.h", "mg_tiles.h", "mg_launch.h"]
@@ -162,5 +163,46 @@ def _build_locked(force, verbose, missing_hipcc_ok, lib, extra_flags, extra_link
     return lib
 
 
+def build_torch_ops(force: bool = False, missing_compiler_ok: bool = False) -> str:
+    """The torch binding of the learning operators: host code only, against the headers of the installed torch, and for that torch alone (its version is
+    part of the stamp).  A no-op where the built one is up to date."""
+    import torch
+    src, stamp = os.path.join("ops", "mg_torch.cpp"), TORCH_OPS + ".srchash"
+    cxx = shutil.which("g++")
+    base = os.path.dirname(torch.__file__)
+    flags = ["-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall", "-DTORCH_EXTENSION_NAME=_torch_ops", "-DTORCH_API_INCLUDE_EXTENSION_H", "-D__HIP_PLATFORM_AMD__=1",
+             "-DUSE_ROCM=1", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    want = _hash_files([src, ABI_HEADER, os.path.join("..", "..", "include", "minigrid_ops.h")], " ".join(flags) + torch.__version__ + sys.version)
+
+    def fresh():
+        return not force and os.path.exists(TORCH_OPS) and os.path.exists(stamp) and open(stamp).read().strip() == want
+    if fresh():
+        return TORCH_OPS
+    if not cxx:
+        if missing_compiler_ok and os.path.exists(TORCH_OPS):
+            return TORCH_OPS
+        raise RuntimeError("g++ not found: cannot build the learning operators' torch binding")
+    import fcntl
+    import sysconfig
+    os.makedirs(OBJDIR, exist_ok=True)
+    with open(os.path.join(OBJDIR, ".lock_torch"), "w") as lock:
+        fcntl.flock(lock, fcntl.LOCK_EX)
+        if fresh():
+            return TORCH_OPS
+        rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
+        include = [os.path.join(base, "include"), os.path.join(base, "include", "torch", "csrc", "api", "include"), os.path.join(rocm, "include"), sysconfig.get_path("include")]
+        out = f"{TORCH_OPS}.{os.getpid()}"               # (a process that has the old one loaded keeps it)
+        subprocess.check_call([cxx] + flags + [a for i in include for a in ("-isystem", i)] + [os.path.join(CSRC, src), "-o", out, "-L" + os.path.join(base, "lib"),
+                              "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-ldl"])
+        os.replace(out, TORCH_OPS)
+        with open(stamp, "w") as f:
+            f.write(want)
+    return TORCH_OPS
+
+
 if __name__ == "__main__":
     print(build(force="--force" in sys.argv, verbose=True))
+    try:
+        print(build_torch_ops(force="--force" in sys.argv))
+    except ImportError:
+        print("no torch: the learning operators' binding is not built")

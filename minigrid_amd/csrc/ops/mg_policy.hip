@@ -11,7 +11,28 @@ namespace mgo {
 constexpr int SMALL_VOCAB = 64;          // up to here a lane owns a row
 constexpr float NEG_INF = -__builtin_inff();
 
-struct Saved { double lse; float dlp, entropy; };       // of a row, for the backward pass: 16 bytes
+// e^d for d <= 0 (or -inf, or NaN) in 64 bits: d = k ln 2 + r with |r| <= ln 2 / 2, e^r as its Taylor sum up to r^12 (what is left out is below 2e-16)
+__device__ __forceinline__ double exp_neg(double d) {
+  const double k = __builtin_rint(d * 1.44269504088896340736);
+  const double r = __builtin_fma(k, -2.3190468138462996e-17, __builtin_fma(k, -LN2, d));     // ln 2 in two parts
+  double p = 1.0 / 479001600.0;
+  p = __builtin_fma(p, r, 1.0 / 39916800.0);
+  p = __builtin_fma(p, r, 1.0 / 3628800.0);
+  p = __builtin_fma(p, r, 1.0 / 362880.0);
+  p = __builtin_fma(p, r, 1.0 / 40320.0);
+  p = __builtin_fma(p, r, 1.0 / 5040.0);
+  p = __builtin_fma(p, r, 1.0 / 720.0);
+  p = __builtin_fma(p, r, 1.0 / 120.0);
+  p = __builtin_fma(p, r, 1.0 / 24.0);
+  p = __builtin_fma(p, r, 1.0 / 6.0);
+  p = __builtin_fma(p, r, 0.5);
+  p = __builtin_fma(p, r, 1.0);
+  p = __builtin_fma(p, r, 1.0);
+  const double e = __builtin_amdgcn_ldexp(p, (int)k);
+  return d < -745.2 ? 0.0 : e;
+}
+
+struct Saved { double lse; float dlp, entropy; };       // of a row, for the backward pass; one more behind the rows holds their number (in lse)
 static_assert(sizeof(Saved) == 16, "the header promises 16 bytes a row");
 
 struct LossArgs {
@@ -44,6 +65,7 @@ __device__ __forceinline__ void row_terms(const LossArgs& a, int64_t i, double l
 }
 
 __device__ __forceinline__ void write_out(const LossArgs& a, const Terms& t, float* out) {
+  if (a.save) a.save[a.rows] = {t.count, 0.0f, 0.0f};
   const double inv = t.count > 0.0 ? 1.0 / t.count : 0.0, p = t.policy * inv, k = t.kl * inv, h = t.entropy * inv;
   out[0] = (float)(p + a.kl * k - a.ent * h); out[1] = (float)p; out[2] = (float)k; out[3] = (float)h; out[4] = (float)(t.clipped * inv); out[5] = (float)t.count;
 }
@@ -52,20 +74,25 @@ __device__ __forceinline__ void wave_sum(Terms& t) {
   t.policy = wave_sum(t.policy); t.kl = wave_sum(t.kl); t.entropy = wave_sum(t.entropy); t.clipped = wave_sum(t.clipped); t.count = wave_sum(t.count);
 }
 
-// the workgroups' sums in their order (each lane its run of them, then the lanes): one workgroup
-__global__ __launch_bounds__(256) void k_loss_out(LossArgs a, int64_t n, const Terms* part, float* out) {
-  __shared__ Terms s[4];
+// partial sums: five arrays of n
+__device__ __forceinline__ void put_part(double* part, int64_t n, int64_t at, const Terms& t) {
+  part[at] = t.policy; part[n + at] = t.kl; part[2 * n + at] = t.entropy; part[3 * n + at] = t.clipped; part[4 * n + at] = t.count;
+}
+
+// the workgroups' sums in their order (each lane every 1024th of them, then the lanes): one workgroup
+__global__ __launch_bounds__(1024) void k_loss_out(LossArgs a, int64_t n, const double* part, float* out) {
+  __shared__ Terms s[16];
   Terms t = {};
-  for (int64_t u = threadIdx.x; u < n; u += 256) {
-    const Terms& p = part[u];
-    t.policy += p.policy; t.kl += p.kl; t.entropy += p.entropy; t.clipped += p.clipped; t.count += p.count;
+#pragma unroll 2
+  for (int64_t u = threadIdx.x; u < n; u += 1024) {
+    t.policy += part[u]; t.kl += part[n + u]; t.entropy += part[2 * n + u]; t.clipped += part[3 * n + u]; t.count += part[4 * n + u];
   }
   wave_sum(t);
   if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = t;
   __syncthreads();
   if (threadIdx.x == 0) {
     Terms r = {};
-    for (int w = 0; w < 4; w++) { r.policy += s[w].policy; r.kl += s[w].kl; r.entropy += s[w].entropy; r.clipped += s[w].clipped; r.count += s[w].count; }
+    for (int w = 0; w < 16; w++) { r.policy += s[w].policy; r.kl += s[w].kl; r.entropy += s[w].entropy; r.clipped += s[w].clipped; r.count += s[w].count; }
     write_out(a, r, out);
   }
 }
@@ -82,7 +109,7 @@ __device__ __forceinline__ void stage_rows(const T* logits, int64_t ld, int64_t 
 
 // few columns: a lane owns a row, 64-bit throughout (seven exponentials a row are nothing)
 template <class T>
-__global__ void k_loss_small(LossArgs a, Terms* part, float* out) {
+__global__ void k_loss_small(LossArgs a, double* part, float* out) {
   extern __shared__ float lds[];
   const int vocab = (int)a.vocab, R = blockDim.x;
   const int64_t first = (int64_t)blockIdx.x * R;
@@ -97,7 +124,7 @@ __global__ void k_loss_small(LossArgs a, Terms* part, float* out) {
     for (int c = 0; c < vocab; c++) m = fmaxf(m, l[c]);
     double s = 0.0, t = 0.0;
     for (int c = 0; c < vocab; c++) {
-      const double d = (double)l[c] - (double)m, e = exp(d);
+      const double d = (double)l[c] - (double)m, e = exp_neg(d);
       s += e;
       t += e == 0.0 ? 0.0 : e * d;                              // a closed column: e^-inf (-inf) counts 0
     }
@@ -115,7 +142,7 @@ __global__ void k_loss_small(LossArgs a, Terms* part, float* out) {
     Terms r = {};
     for (int v = 0; v < R / 64; v++) { r.policy += w[v].policy; r.kl += w[v].kl; r.entropy += w[v].entropy; r.clipped += w[v].clipped; r.count += w[v].count; }
     if (gridDim.x == 1) write_out(a, r, out);
-    else part[blockIdx.x] = r;
+    else put_part(part, gridDim.x, blockIdx.x, r);
   }
 }
 
@@ -125,7 +152,7 @@ struct Sums { float m; double s, t; };
 __device__ __forceinline__ void join(Sums& a, float m, double s, double t) {      // a += (m, s, t)
   const float M = fmaxf(a.m, m);
   const double da = a.m == NEG_INF ? 0.0 : (double)a.m - (double)M, db = m == NEG_INF ? 0.0 : (double)m - (double)M;      // (a part without a finite logit has s = t = 0)
-  const double fa = exp(da), fb = exp(db);
+  const double fa = exp_neg(da), fb = exp_neg(db);
   a.t = fa * (a.t + da * a.s) + fb * (t + db * s);
   a.s = fa * a.s + fb * s;
   a.m = M;
@@ -138,7 +165,7 @@ __device__ __forceinline__ void add_chunk(Sums& a, const float (&x)[N]) {
   for (int u = 1; u < N; u++) top = fmaxf(top, x[u]);
   if (top > a.m) {
     if (a.s != 0.0) {
-      const double d = (double)a.m - (double)top, f = exp(d);
+      const double d = (double)a.m - (double)top, f = exp_neg(d);
       a.t = f * (a.t + d * a.s);
       a.s = f * a.s;
     }
@@ -150,17 +177,21 @@ __device__ __forceinline__ void add_chunk(Sums& a, const float (&x)[N]) {
       if (x[u] != x[u]) a.s = a.t = __builtin_nan("");
     return;
   }
-  float s = 0.0f, t = 0.0f;                                      // eight terms in 32 bits, then into the 64-bit sum
+  constexpr int G = N < 8 ? N : 8;
 #pragma unroll
-  for (int u = 0; u < N; u++) {
-    float d = x[u] - a.m;
-    d = d < -200.0f ? -200.0f : d;                               // e^-200 is 0 in 32 bits, and 0 * -200 is 0 (keeps a NaN)
-    const float e = __builtin_amdgcn_exp2f(d * LOG2E_HI);
-    s += e;
-    t = __builtin_fmaf(e, d, t);
+  for (int g = 0; g < N; g += G) {
+    float s = 0.0f, t = 0.0f;                                    // eight terms in 32 bits, then into the 64-bit sum
+#pragma unroll
+    for (int u = g; u < g + G; u++) {
+      float d = x[u] - a.m;
+      d = d < -200.0f ? -200.0f : d;                             // e^-200 is 0 in 32 bits, and 0 * -200 is 0 (keeps a NaN)
+      const float e = __builtin_amdgcn_exp2f(d * LOG2E_HI);
+      s += e;
+      t = __builtin_fmaf(e, d, t);
+    }
+    a.s += (double)s;
+    a.t += (double)t;
   }
-  a.s += (double)s;
-  a.t += (double)t;
 }
 
 template <class T> struct Pack { static constexpr int N = 16 / sizeof(T); };
@@ -173,7 +204,17 @@ __device__ __forceinline__ Sums row_sums(const T* row, int64_t from, int64_t to,
   const int64_t skew = (int64_t)(((uintptr_t)(row + from) & 15) / sizeof(T));
   const int64_t head = min(to, from + (skew ? N - skew : 0)), body = head + (to - head) / N * N;
   if (from + tid < head) { const float x[1] = {(float)row[from + tid]}; add_chunk(a, x); }
-  for (int64_t c = head + (int64_t)tid * N; c < body; c += (int64_t)NT * N) {
+  int64_t c = head + (int64_t)tid * N;
+  for (; c + 3 * NT * N < body; c += (int64_t)4 * NT * N) {       // four chunks on their way at a time, one look at the maximum
+    T v[4][N];
+#pragma unroll
+    for (int g = 0; g < 4; g++) __builtin_memcpy(v[g], __builtin_assume_aligned(row + c + g * NT * N, 16), 16);
+    float x[4 * N];
+#pragma unroll
+    for (int u = 0; u < 4 * N; u++) x[u] = (float)v[u / N][u % N];
+    add_chunk(a, x);
+  }
+  for (; c < body; c += (int64_t)NT * N) {
     T v[N];
     __builtin_memcpy(v, __builtin_assume_aligned(row + c, 16), 16);
     float x[N];
@@ -187,7 +228,7 @@ __device__ __forceinline__ Sums row_sums(const T* row, int64_t from, int64_t to,
 
 __device__ __forceinline__ void wave_join(Sums& a) {
   const float M = wave_max(a.m);
-  const double d = a.m == NEG_INF ? 0.0 : (double)a.m - (double)M, f = exp(d);
+  const double d = a.m == NEG_INF ? 0.0 : (double)a.m - (double)M, f = exp_neg(d);
   a.t = wave_sum(f * (a.t + d * a.s));
   a.s = wave_sum(f * a.s);
   a.m = M;
@@ -195,7 +236,7 @@ __device__ __forceinline__ void wave_join(Sums& a) {
 
 // a workgroup per row
 template <class T>
-__global__ __launch_bounds__(256) void k_loss_rows(LossArgs a, Terms* part) {
+__global__ __launch_bounds__(256) void k_loss_rows(LossArgs a, double* part) {
   __shared__ Sums w[4];
   const int64_t i = blockIdx.x;
   Terms sum = {};
@@ -212,13 +253,13 @@ __global__ __launch_bounds__(256) void k_loss_rows(LossArgs a, Terms* part) {
       row_terms(a, i, (double)s.m + ls, ls - s.t / s.s, act >= 0 && act < a.vocab ? (double)(float)row[act] : __builtin_nan(""), sum);
     }
   }
-  if (threadIdx.x == 0) part[i] = sum;
+  if (threadIdx.x == 0) put_part(part, a.rows, i, sum);
 }
 
 // d loss / d logit_j = g / count (dlp (1[j = action] - p_j) + ent p_j (l_j - lse + H)), p_j = e^{l_j - lse}
 struct GradArgs {
   const void* logits; int64_t ld; const void* action; int32_t action_dtype; const uint8_t* mask;
-  const Saved* save; const float *out, *grad; void* dlogits;
+  const Saved* save; const float* grad; void* dlogits;
   float ent; int64_t rows, vocab;
 };
 __device__ __forceinline__ float grad_of(float l, double lse, float entropy, float dlp, float ent, bool chosen) {
@@ -241,7 +282,7 @@ __global__ void k_grad_small(GradArgs a) {
     const int64_t i = first + threadIdx.x;
     if (!a.mask || a.mask[i]) {
       const Saved s = a.save[i];
-      const float share = a.grad[0] / a.out[5], dlp = s.dlp * share, ent = a.ent * share;
+      const float share = a.grad[0] / (float)a.save[a.rows].lse, dlp = s.dlp * share, ent = a.ent * share;
       const int64_t act = action_of(a, i);
       for (int c = 0; c < vocab; c++) l[c] = grad_of(l[c], s.lse, s.entropy, dlp, ent, c == act);
     } else {
@@ -261,7 +302,8 @@ constexpr int64_t GRAD_RUN = 16384;      // elements of a row per workgroup
 template <class T>
 __global__ __launch_bounds__(256) void k_grad_rows(GradArgs a) {
   constexpr int N = Pack<T>::N;
-  const int64_t i = blockIdx.x, from = (int64_t)blockIdx.y * GRAD_RUN, to = min(a.vocab, from + GRAD_RUN);
+  // (the last rows first: the forward pass has just left them in the cache behind the L2s)
+  const int64_t i = a.rows - 1 - (int64_t)blockIdx.x, from = (int64_t)blockIdx.y * GRAD_RUN, to = min(a.vocab, from + GRAD_RUN);
   const bool on = !a.mask || a.mask[i];
   const T* row = (const T*)a.logits + i * a.ld;
   T* d = (T*)a.dlogits + i * a.vocab;
@@ -270,7 +312,7 @@ __global__ __launch_bounds__(256) void k_grad_rows(GradArgs a) {
   int64_t act = -1;
   if (on) {
     s = a.save[i];
-    const float share = a.grad[0] / a.out[5];
+    const float share = a.grad[0] / (float)a.save[a.rows].lse;
     dlp = s.dlp * share; ent = a.ent * share; act = action_of(a, i);
   }
   // whole 16-byte stores: the run is counted from the gradient's alignment, the logits may lie at any
@@ -312,7 +354,7 @@ __global__ void k_sample_small(const T* logits, int64_t ld, int64_t rows_all, in
   for (int c = 0; c < vocab; c++)
     if (l[c] > m) { m = l[c]; best = c; }
   double s = 0.0;
-  for (int c = 0; c < vocab; c++) s += exp((double)l[c] - (double)m);
+  for (int c = 0; c < vocab; c++) s += exp_neg((double)l[c] - (double)m);
   int k = best;
   if (u) {
     const double target = (double)u[i] * s;
@@ -320,7 +362,7 @@ __global__ void k_sample_small(const T* logits, int64_t ld, int64_t rows_all, in
     int last = 0;
     k = -1;
     for (int c = 0; c < vocab && k < 0; c++) {
-      const double e = exp((double)l[c] - (double)m);
+      const double e = exp_neg((double)l[c] - (double)m);
       run += e;
       if (e > 0.0) { last = c; if (run > target) k = c; }
     }
@@ -331,112 +373,157 @@ __global__ void k_sample_small(const T* logits, int64_t ld, int64_t rows_all, in
   lp[i] = fine ? (float)((double)l[k] - (double)m - log(s)) : __builtin_nanf("");
 }
 
-// A workgroup of sixteen waves per row; a wave owns one contiguous sixteenth.  Pass 1: the maximum; pass 2: the waves' sums; then the one wave whose
-// part holds the border walks it, 64 lanes x 8 elements at a time.
+// Long rows: a row is cut into 64 pieces, a wave per piece finds its maximum and its sum against it; from the 64 pairs one wave finds the piece in which the
+// running sum passes the border, and walks that piece alone.  Few rows: the pieces of a row are dealt to up to sixteen workgroups, and a second kernel
+// walks; many rows: one workgroup of four waves does both.  Bound by memory for many rows, by two short launches for few.
+constexpr int PIECES = 64, E = 4;        // E: elements of a lane at a time
+struct Piece { float m; int32_t at; double s; };          // the largest logit, its first index, sum e^{l - m}
+static_assert(sizeof(Piece) == 16, "the workspace is counted in these");
+
+__device__ __forceinline__ int64_t piece_length(int64_t vocab) { return ((vocab + PIECES - 1) / PIECES + E - 1) / E * E; }
+
 template <class T>
-__global__ __launch_bounds__(1024) void k_sample_rows(const T* logits, int64_t ld, int64_t vocab, const float* u, void* action, float* lp) {
-  __shared__ float wm[16];
-  __shared__ int64_t wi[16];
-  __shared__ double ws[16];
-  __shared__ int64_t wl[16];
-  constexpr int E = 8;
-  const int64_t i = blockIdx.x;
-  const T* row = logits + i * ld;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int64_t run = ((vocab + 15) / 16 + 64 * E - 1) / (64 * E) * (64 * E), from = min(vocab, w * run), to = min(vocab, from + run);
+__device__ __forceinline__ void load_some(const T* row, int64_t c, int64_t to, float (&x)[E]) {
+  if (c + E <= to) {
+    T v[E];
+    __builtin_memcpy(v, row + c, sizeof v);
+#pragma unroll
+    for (int q = 0; q < E; q++) x[q] = (float)v[q];
+  } else {
+#pragma unroll
+    for (int q = 0; q < E; q++) x[q] = c + q < to ? (float)row[c + q] : NEG_INF;
+  }
+}
+
+template <class T>
+__device__ __forceinline__ Piece look_at(const T* row, int64_t from, int64_t to) {
+  const int lane = threadIdx.x & 63;
   float m = NEG_INF;
-  int64_t at = vocab;
-  for (int64_t c = from + lane; c < to; c += 64) {
-    const float x = (float)row[c];
-    if (x > m) { m = x; at = c; }
-  }
-  const float M0 = wave_max(m);
-  int64_t a0 = m == M0 && m != NEG_INF ? at : vocab;
-#pragma unroll
-  for (int b = 32; b; b >>= 1) {
-    const int64_t o = (int64_t)(uint32_t)__shfl_xor((int)(uint32_t)a0, b) | (int64_t)__shfl_xor((int)(a0 >> 32), b) << 32;
-    a0 = min(a0, o);
-  }
-  if (lane == 0) { wm[w] = M0; wi[w] = a0; }
-  __syncthreads();
-  float M = wm[0];
-  int64_t best = wi[0];
-  for (int v = 1; v < 16; v++)
-    if (wm[v] > M) { M = wm[v]; best = wi[v]; }
+  int64_t at = to;
   double s = 0.0;
-  int64_t last = -1;
-  for (int64_t c = from + lane; c < to; c += 64) {
-    const double e = exp((double)(float)row[c] - (double)M);
-    s += e;
-    if (e > 0.0) last = c;
-  }
-  s = wave_sum(s);
+#pragma unroll 2
+  for (int64_t c0 = from; c0 < to; c0 += 64 * E) {
+    const int64_t c = c0 + lane * E;
+    float x[E];
+    load_some(row, c, to, x);
+    float top = m;
 #pragma unroll
-  for (int b = 32; b; b >>= 1) {
-    const int64_t o = (int64_t)(uint32_t)__shfl_xor((int)(uint32_t)last, b) | (int64_t)__shfl_xor((int)(last >> 32), b) << 32;
-    last = max(last, o);
+    for (int q = 0; q < E; q++)
+      if (x[q] > top) { top = x[q]; at = c + q; }
+    const double M = top == NEG_INF ? 0.0 : (double)top;
+    s *= m == NEG_INF ? 1.0 : exp_neg((double)m - M);            // (without a finite logit so far the sum is 0 or NaN)
+#pragma unroll
+    for (int q = 0; q < E; q++) s += exp_neg((double)x[q] - M);
+    m = top;
   }
-  if (lane == 0) { ws[w] = s; wl[w] = last; }
-  __syncthreads();
-  double S = 0.0;
-  for (int v = 0; v < 16; v++) S += ws[v];
-  const bool fine = S > 0.0 && S < __builtin_inf();
-  if (!fine) {
-    if (threadIdx.x == 0) { store_action(action, vocab, i, 0); lp[i] = __builtin_nanf(""); }
+  const float M = wave_max(m);
+  int first = m == M && m != NEG_INF ? (int)(at - from) : 0x7fffffff;
+#pragma unroll
+  for (int b = 32; b; b >>= 1) first = min(first, __shfl_xor(first, b));
+  s = wave_sum(s * (m == NEG_INF ? 1.0 : exp_neg((double)m - (double)M)));
+  return {M, (int32_t)(from + first), s};
+}
+
+// by one wave, lane q with the row's piece q
+template <class T>
+__device__ __forceinline__ void choose(const T* row, int64_t vocab, Piece mine, int64_t i, const float* u, void* action, float* lp) {
+  const int lane = threadIdx.x & 63;
+  const float M = wave_max(mine.m);
+  const double share = mine.s * (mine.m == NEG_INF ? 1.0 : exp_neg((double)mine.m - (double)M));
+  double upto = share;                                           // inclusive over the pieces
+#pragma unroll
+  for (int b = 1; b < 64; b <<= 1) {
+    const double o = __hiloint2double(__shfl_up(__double2hiint(upto), b), __shfl_up(__double2loint(upto), b));
+    if (lane >= b) upto += o;
+  }
+  auto of_lane = [](double v, int l) { return __hiloint2double(__shfl(__double2hiint(v), l), __shfl(__double2loint(v), l)); };
+  const double S = of_lane(upto, 63);
+  if (!(S > 0.0 && S < __builtin_inf())) {                       // (false for NaN)
+    if (lane == 0) { store_action(action, vocab, i, 0); lp[i] = __builtin_nanf(""); }
     return;
   }
-  int64_t k = best;
+  int64_t k = __shfl(mine.at, __ffsll((long long)__ballot(mine.m == M)) - 1);
   if (u) {
     const double target = (double)u[i] * S;
-    double before = 0.0;
-    int mine = -1;
-    int64_t end = 0;
-    for (int v = 0; v < 16; v++) {
-      if (wl[v] >= 0) { end = wl[v]; if (before + ws[v] > target) { mine = v; break; } }
-      before += ws[v];
-    }
-    k = end;                                                     // u s was reached by rounding only: the last element that has a share
-    if (mine >= 0) {
-      if (w != mine) return;
-      bool found = false;
-      for (int64_t c0 = from; c0 < to && !found; c0 += 64 * E) {
-        double e[E], sum = 0.0;
+    const int64_t len = piece_length(vocab);
+    const unsigned long long over = __ballot(upto > target && share > 0.0), some = __ballot(share > 0.0);
+    // beyond every piece by rounding only: the last element that has a share, in the last piece that has one
+    const int p = over ? __ffsll((long long)over) - 1 : 63 - __builtin_clzll(some);
+    double before = p ? of_lane(upto, p - 1) : 0.0;
+    const int64_t from = p * len, to = min(vocab, from + len);
+    int64_t last = -1;
+    bool found = false;
+    for (int64_t c0 = from; c0 < to && !found; c0 += 64 * E) {
+      float x[E];
+      load_some(row, c0 + lane * E, to, x);
+      double e[E], sum = 0.0;
 #pragma unroll
-        for (int q = 0; q < E; q++) {
-          const int64_t c = c0 + lane * E + q;
-          e[q] = c < to ? exp((double)(float)row[c] - (double)M) : 0.0;
-          sum += e[q];
-        }
-        double upto = sum;                                       // inclusive over the lanes
+      for (int q = 0; q < E; q++) { e[q] = exp_neg((double)x[q] - (double)M); sum += e[q]; }
+      double run = sum;
 #pragma unroll
-        for (int b = 1; b < 64; b <<= 1) {
-          const double o = __hiloint2double(__shfl_up(__double2hiint(upto), b), __shfl_up(__double2loint(upto), b));
-          if (lane >= b) upto += o;
-        }
-        const unsigned long long hit = __ballot(before + upto > target && sum > 0.0);
-        if (hit) {
-          found = true;
-          if (lane == __ffsll((long long)hit) - 1) {
-            double r = before + (upto - sum);
-            int64_t pick = -1, some = -1;
-#pragma unroll
-            for (int q = 0; q < E; q++) {
-              r += e[q];
-              if (e[q] > 0.0) { some = c0 + lane * E + q; if (pick < 0 && r > target) pick = some; }
-            }
-            k = pick >= 0 ? pick : some;
-            store_action(action, vocab, i, k);
-            lp[i] = (float)((double)(float)row[k] - (double)M - log(S));
-          }
-        }
-        before += __hiloint2double(__shfl(__double2hiint(upto), 63), __shfl(__double2loint(upto), 63));
+      for (int b = 1; b < 64; b <<= 1) {
+        const double o = __hiloint2double(__shfl_up(__double2hiint(run), b), __shfl_up(__double2loint(run), b));
+        if (lane >= b) run += o;
       }
-      if (found) return;
-      if (lane) return;
-    } else if (threadIdx.x) return;
-  } else if (threadIdx.x) return;
-  store_action(action, vocab, i, k);
-  lp[i] = (float)((double)(float)row[k] - (double)M - log(S));
+      // the running sum as the lane's elements see it: exact enough to be compared lane by lane, and what a lane passes is passed by its last element
+      double r = before + (run - sum);
+      int pick = -1, any = -1;
+#pragma unroll
+      for (int q = 0; q < E; q++) {
+        r += e[q];
+        if (e[q] > 0.0) { any = q; if (pick < 0 && r > target) pick = q; }
+      }
+      const unsigned long long hit = __ballot(pick >= 0), has = __ballot(any >= 0);
+      if (hit) {
+        const int w = __ffsll((long long)hit) - 1;
+        last = c0 + w * E + __shfl(pick, w);
+        found = true;
+      } else if (has) {
+        const int w = 63 - __builtin_clzll(has);
+        last = c0 + w * E + __shfl(any, w);
+      }
+      before += of_lane(run, 63);
+    }
+    if (last >= 0) k = last;
+  }
+  if (lane == 0) {
+    store_action(action, vocab, i, k);
+    lp[i] = (float)((double)(float)row[k] - (double)M - log(S));
+  }
+}
+
+// grid (rows, groups): group g looks at its 64 / groups pieces of a row; a single group chooses at once
+template <class T>
+__global__ __launch_bounds__(256) void k_sample_rows(const T* logits, int64_t ld, int64_t vocab, const float* u, Piece* pieces, void* action, float* lp) {
+  __shared__ Piece all[PIECES];
+  const int64_t i = blockIdx.x;
+  const T* row = logits + i * ld;
+  const int w = threadIdx.x >> 6, n = PIECES / gridDim.y, first = blockIdx.y * n;
+  const int64_t len = piece_length(vocab);
+  for (int p = first + w; p < first + n; p += 4) {
+    const int64_t from = min(vocab, p * len), to = min(vocab, from + len);
+    const Piece q = look_at(row, from, to);
+    if ((threadIdx.x & 63) == 0) {
+      if (pieces) pieces[i * PIECES + p] = q;
+      else all[p] = q;
+    }
+  }
+  if (pieces) return;
+  __syncthreads();
+  if (w == 0) choose(row, vocab, all[threadIdx.x & 63], i, u, action, lp);
+}
+
+template <class T>
+__global__ __launch_bounds__(64) void k_sample_choose(const T* logits, int64_t ld, int64_t vocab, const float* u, const Piece* pieces, void* action, float* lp) {
+  const int64_t i = blockIdx.x;
+  choose(logits + i * ld, vocab, pieces[i * PIECES + threadIdx.x], i, u, action, lp);
+}
+
+// workgroups per row: enough of them for every CU, each of its four waves with at least one piece
+static int sample_groups(int64_t rows) {
+  int g = 1;
+  while (g < PIECES / 4 && rows * g < 512) g *= 2;
+  return g;
 }
 
 static int check_logits(int dtype, int64_t rows, int64_t vocab, int64_t ld) {
@@ -489,7 +576,7 @@ int mg_op_policy_loss(int device, void* stream, int dtype, int64_t rows, int64_t
     parts = (rows + R - 1) / R;
     by_type(dtype, [&](auto* t) {
       typedef std::remove_cv_t<std::remove_pointer_t<decltype(t)>> T;
-      k_loss_small<T><<<(unsigned)parts, R, small_lds(R, vocab), st>>>(a, (Terms*)ws, out);
+      k_loss_small<T><<<(unsigned)parts, R, small_lds(R, vocab), st>>>(a, (double*)ws, out);
       return 0;
     });
     if (parts == 1) return launched("policy loss");
@@ -497,24 +584,24 @@ int mg_op_policy_loss(int device, void* stream, int dtype, int64_t rows, int64_t
     parts = rows;
     by_type(dtype, [&](auto* t) {
       typedef std::remove_cv_t<std::remove_pointer_t<decltype(t)>> T;
-      k_loss_rows<T><<<(unsigned)rows, 256, 0, st>>>(a, (Terms*)ws);
+      k_loss_rows<T><<<(unsigned)rows, 256, 0, st>>>(a, (double*)ws);
       return 0;
     });
   }
-  k_loss_out<<<1, 256, 0, st>>>(a, parts, (const Terms*)ws, out);
+  k_loss_out<<<1, 1024, 0, st>>>(a, parts, (const double*)ws, out);
   return launched("policy loss");
 }
 
 int mg_op_policy_loss_backward(int device, void* stream, int dtype, int64_t rows, int64_t vocab, const void* logits, int64_t ld, const void* action, int action_dtype,
-                               const uint8_t* mask, double ent_coef, const float* out, const void* save, const float* grad, void* dlogits) {
+                               const uint8_t* mask, double ent_coef, const void* save, const float* grad, void* dlogits) {
   int rc = check_logits(dtype, rows, vocab, ld);
   if (rc == MG_OK) rc = check_action(action_dtype);
   if (rc != MG_OK || rows == 0) return rc;
-  if (!logits || !action || !out || !save || !grad || !dlogits) return fail(MG_ERR_INVALID, "no pointer but mask may be NULL");
+  if (!logits || !action || !save || !grad || !dlogits) return fail(MG_ERR_INVALID, "no pointer but mask may be NULL");
   DeviceGuard g(device);
   if (g.rc != MG_OK) return g.rc;
   hipStream_t st = (hipStream_t)stream;
-  GradArgs a = {logits, ld, action, action_dtype, mask, (const Saved*)save, out, grad, dlogits, (float)ent_coef, rows, vocab};
+  GradArgs a = {logits, ld, action, action_dtype, mask, (const Saved*)save, grad, dlogits, (float)ent_coef, rows, vocab};
   return by_type(dtype, [&](auto* t) {
     typedef std::remove_cv_t<std::remove_pointer_t<decltype(t)>> T;
     if (vocab <= SMALL_VOCAB) {
@@ -529,20 +616,36 @@ int mg_op_policy_loss_backward(int device, void* stream, int dtype, int64_t rows
   });
 }
 
-int mg_op_sample(int device, void* stream, int dtype, int64_t rows, int64_t vocab, const void* logits, int64_t ld, const float* u, void* action, float* lp) {
+int mg_op_sample_workspace(int64_t rows, int64_t vocab, int64_t* bytes) {
+  const int rc = check_logits(MG_DT_F32, rows, vocab, vocab);
+  if (rc != MG_OK) return rc;
+  if (!bytes) return fail(MG_ERR_INVALID, "bytes must not be NULL");
+  *bytes = vocab > SMALL_VOCAB && sample_groups(rows) > 1 ? rows * PIECES * (int64_t)sizeof(Piece) : 0;
+  return MG_OK;
+}
+
+int mg_op_sample(int device, void* stream, int dtype, int64_t rows, int64_t vocab, const void* logits, int64_t ld, const float* u, void* action, float* lp, void* ws,
+                 int64_t ws_bytes) {
   int rc = check_logits(dtype, rows, vocab, ld);
   if (rc != MG_OK || rows == 0) return rc;
   if (!logits || !action || !lp) return fail(MG_ERR_INVALID, "logits, action and lp must not be NULL");
+  int64_t need = 0;
+  mg_op_sample_workspace(rows, vocab, &need);
+  if (need && (ws_bytes < need || !ws || ((uintptr_t)ws & 255))) return fail(MG_ERR_INVALID, "workspace: %lld bytes, 256-byte aligned, are needed", (long long)need);
   DeviceGuard g(device);
   if (g.rc != MG_OK) return g.rc;
   hipStream_t st = (hipStream_t)stream;
   return by_type(dtype, [&](auto* t) {
     typedef std::remove_cv_t<std::remove_pointer_t<decltype(t)>> T;
+    const T* x = (const T*)logits;
     if (vocab <= SMALL_VOCAB) {
       const int R = small_rows(vocab);
-      k_sample_small<T><<<(unsigned)((rows + R - 1) / R), R, (size_t)R * (vocab | 1) * 4, st>>>((const T*)logits, ld, rows, (int)vocab, u, action, lp);
+      k_sample_small<T><<<(unsigned)((rows + R - 1) / R), R, (size_t)R * (vocab | 1) * 4, st>>>(x, ld, rows, (int)vocab, u, action, lp);
     } else {
-      k_sample_rows<T><<<(unsigned)rows, 1024, 0, st>>>((const T*)logits, ld, vocab, u, action, lp);
+      const int groups = sample_groups(rows);
+      Piece* pieces = groups > 1 ? (Piece*)ws : nullptr;
+      k_sample_rows<T><<<dim3((unsigned)rows, groups), 256, 0, st>>>(x, ld, vocab, u, pieces, action, lp);
+      if (pieces) k_sample_choose<T><<<(unsigned)rows, 64, 0, st>>>(x, ld, vocab, u, pieces, action, lp);
     }
     return launched("sample");
   });

@@ -635,6 +635,77 @@ def test_captured_and_replayed():
             assert all(torch.equal(p, q) for p, q in zip(want, out)), i
 
 
+@pytest.mark.parametrize("op", ["linear", "policy_loss"])
+def test_capture_beside_an_eager_graph_of_the_same_leaves_is_refused(op):
+    """(the backward pass would end the process)"""
+    x, a, old, adv, ref, mask = loss_inputs(40, 7, torch.float32, 3)
+    x = x.contiguous().requires_grad_(True)
+    w = torch.randn((5, 7), generator=gen(1), device="cuda", requires_grad=True)
+    step = (lambda: mg().linear(x, w, activation="tanh")) if op == "linear" else (lambda: mg().policy_loss(x, a, old, adv)[0])
+    alive = step()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with pytest.raises(ValueError, match="outside of this capture"):
+        with torch.cuda.graph(g):
+            step()
+    del alive, g
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = step()
+        d, = torch.autograd.grad(y.sum(), [x])
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(d, torch.autograd.grad(step().sum(), [x])[0])
+
+
+def test_second_derivatives_are_refused():
+    x, a, old, adv, ref, mask = loss_inputs(40, 7, torch.float32, 3)
+    x = x.contiguous().requires_grad_(True)
+    w = torch.randn((5, 7), generator=gen(1), device="cuda", requires_grad=True)
+    for y in (mg().linear(x, w, activation="tanh").square().sum(), mg().policy_loss(x, a, old, adv)[0]):
+        d, = torch.autograd.grad(y, [x], create_graph=True)
+        with pytest.raises(RuntimeError, match="not differentiable"):
+            torch.autograd.grad(d.sum(), [x])
+
+
+def test_changes_in_place_between_the_passes_are_noticed():
+    x, a, old, adv, ref, mask = loss_inputs(40, 7, torch.float32, 3)
+    w = torch.randn((5, 7), generator=gen(1), device="cuda", requires_grad=True)
+    x = x.contiguous()
+    y = mg().linear(x, w)
+    x.add_(1)
+    with pytest.raises(RuntimeError, match="inplace"):
+        torch.autograd.grad(y.sum(), [w])
+    L = x.clone().requires_grad_(True)
+    loss, stats = mg().policy_loss(L, a, old, adv)
+    want, = torch.autograd.grad(loss, [L], retain_graph=True)
+    stats.zero_()                                                    # (what was returned is the caller's)
+    got, = torch.autograd.grad(loss, [L], retain_graph=True)
+    assert torch.equal(got, want)
+    a.zero_()
+    with pytest.raises(RuntimeError, match="inplace"):
+        torch.autograd.grad(loss, [L])
+    loss = mg().policy_loss(L, a, old, adv)[0]
+    torch.autograd.grad(loss, [L])
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(loss, [L])
+
+
+def test_saved_tensor_hooks_and_checkpointing():
+    """what the backward pass keeps goes through torch's hooks: recomputed, or moved to the host and back, the gradients are the same"""
+    x, w, b, r, dy = linear_inputs(50, 24, 40, torch.bfloat16, False, True, True, False, 5)
+    for t in (x, w, b, r):
+        t.requires_grad_(True)
+    f = lambda: mg().linear(x, w, b, activation="gelu", residual=r)
+    want = torch.autograd.grad(f(), [x, w, b, r], dy)
+    with torch.autograd.graph.save_on_cpu():
+        y = f()
+    assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(y, [x, w, b, r], dy), want))
+    from torch.utils.checkpoint import checkpoint
+    y = checkpoint(lambda *t: mg().linear(t[0], t[1], t[2], activation="gelu", residual=t[3]), x, w, b, r, use_reentrant=False)
+    assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(y, [x, w, b, r], dy), want))
+
+
 # ---- refusals ---------------------------------------------------------------------------------------------------------------------------
 
 def test_refusals():

@@ -71,7 +71,7 @@ def test_c_entries_refuse_before_the_device_is_touched():
     _rc(lin(r=p, ldr=7), "row stride")
     assert lin(rows=0) == B.MG_OK
     need = C.c_int64()
-    assert L.mg_op_linear_workspace(4, 4096, 8, 0, C.byref(need), None, None) == B.MG_OK and need.value > 0
+    assert L.mg_op_linear_workspace(40, 4096, 8, 0, C.byref(need), None, None) == B.MG_OK and need.value > 0
     _rc(L.mg_op_linear_dz(0, None, 0, 3, 4, 8, p, 8, None, p, None, None, 0), "in front of the activation")
     _rc(L.mg_op_linear_dz(0, None, 0, 0, 4, 8, p, 7, None, p, None, None, 0), "row stride")
     _rc(L.mg_op_linear_dx(0, None, 0, 4, 8, 8, p, 8, None, 8, p, None, 0), "NULL")
@@ -85,10 +85,11 @@ def test_c_entries_refuse_before_the_device_is_touched():
     _rc(loss(action=None), "must not be NULL")
     _rc(loss(ws=None), "workspace")
     _rc(loss(wsb=8), "workspace")
-    _rc(L.mg_op_policy_loss_backward(0, None, 0, 4, 7, p, 7, p, 6, None, 0.0, p, None, p, p), "NULL")
-    _rc(L.mg_op_sample(0, None, 0, 4, 7, p, 6, None, p, p), "row stride")
-    _rc(L.mg_op_sample(0, None, 0, 4, 7, p, 7, None, None, p), "NULL")
-    assert L.mg_op_sample(0, None, 0, 0, 7, None, 7, None, None, None) == B.MG_OK
+    _rc(L.mg_op_policy_loss_backward(0, None, 0, 4, 7, p, 7, p, 6, None, 0.0, None, p, p), "NULL")
+    _rc(L.mg_op_sample(0, None, 0, 4, 7, p, 6, None, p, p, None, 0), "row stride")
+    _rc(L.mg_op_sample(0, None, 0, 4, 7, p, 7, None, None, p, None, 0), "NULL")
+    _rc(L.mg_op_sample(0, None, 0, 4, 300, p, 300, None, p, p, None, 0), "workspace")
+    assert L.mg_op_sample(0, None, 0, 0, 7, None, 7, None, None, None, None, 0) == B.MG_OK
     _rc(L.mg_op_advantages(0, None, None), "args")
     a = ops._AdvantagesArgs(steps=2, envs=3)
     _rc(L.mg_op_advantages(0, None, C.byref(a)), "NULL")
@@ -105,4 +106,4 @@ def test_without_a_device_the_entries_say_so():
     if B.load().mg_device_count() > 0:
         pytest.skip("GPU present")
     p = 4096
-    assert ops._lib().mg_op_sample(0, None, 0, 4, 7, p, 7, None, p, p) == B.MG_ERR_NO_DEVICE
+    assert ops._lib().mg_op_sample(0, None, 0, 4, 7, p, 7, None, p, p, None, 0) == B.MG_ERR_NO_DEVICE
