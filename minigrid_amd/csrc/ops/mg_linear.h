@@ -42,7 +42,6 @@ struct Epilogue {
   float* part;     // split sums: f32 (splits, rows, n), contiguous; null = store the result
   int64_t ldr, ldc;
   int32_t act;
-  int32_t wide;    // n and every row stride divide by 8 and every pointer by 16 bytes
 };
 
 // ---- activations ----
@@ -253,52 +252,43 @@ __device__ __forceinline__ f32x16 mma(f32x4 a, f32x4 b, f32x16 c) {   // both op
   return c;
 }
 
-// W consecutive elements (i, j ..) of the result, those from `skip` up to `count` to be stored; the sums come in 32 bits and each result is rounded to T once.  WIDE: all of
-// them inside and every row 16-byte aligned.
-template <class T, int W, bool WIDE>
-__device__ __forceinline__ void finish(const Epilogue& e, int64_t i, int64_t j, int64_t n, int skip, int count, float (&v)[W]) {
+// one element of the result; the sum comes in 32 bits and each result is rounded to T once
+template <class T> __device__ __forceinline__ float activate_any(int act, float z) {
+  switch (act) {
+    case MG_ACTIVATION_RELU: return activate(MG_ACTIVATION_RELU, z);
+    case MG_ACTIVATION_TANH: return activate(MG_ACTIVATION_TANH, z);
+    case MG_ACTIVATION_GELU: return activate(MG_ACTIVATION_GELU, z);
+    case MG_ACTIVATION_SILU: return activate(MG_ACTIVATION_SILU, z);
+    default: return z;
+  }
+}
+template <class T>
+__device__ __forceinline__ void finish(const Epilogue& e, int64_t i, int64_t j, int64_t n, float v) {
+  if (e.b) v += (float)((const T*)e.b)[j];
+  if (e.z) ((T*)e.z)[i * n + j] = (T)v;
+  v = activate_any<T>(e.act, v);
+  if (e.r) v += (float)((const T*)e.r)[i * e.ldr + j];
+  ((T*)e.c)[i * e.ldc + j] = (T)v;
+}
+
+// W neighbours of a row at any alignment, those from `skip` up to `count`
+template <class T, int W>
+__device__ __forceinline__ void store_some(T* p, const float (&v)[W], int skip, int count) {
   T t[W];
-  if (e.b) {
-#pragma unroll
-    for (int u = 0; u < W; u++)
-      if (WIDE || u < count) v[u] += (float)((const T*)e.b)[j + u];
-  }
-  if (e.z) {
-    T* z = (T*)e.z + i * n + j;
-#pragma unroll
-    for (int u = 0; u < W; u++) t[u] = (T)v[u];
-    if constexpr (WIDE) __builtin_memcpy(__builtin_assume_aligned(z, 16), t, sizeof t);
-    else
-#pragma unroll
-      for (int u = 0; u < W; u++)
-        if (u >= skip && u < count) z[u] = t[u];
-  }
-  switch (e.act) {
-#define MG_ACT(A) case A: _Pragma("unroll") for (int u = 0; u < W; u++) v[u] = activate(A, v[u]); break;
-    MG_ACT(MG_ACTIVATION_RELU) MG_ACT(MG_ACTIVATION_TANH) MG_ACT(MG_ACTIVATION_GELU) MG_ACT(MG_ACTIVATION_SILU)
-#undef MG_ACT
-    default: break;
-  }
-  if (e.r) {
-    const T* r = (const T*)e.r + i * e.ldr + j;
-    if constexpr (WIDE) {
-      __builtin_memcpy(t, __builtin_assume_aligned(r, 16), sizeof t);
-#pragma unroll
-      for (int u = 0; u < W; u++) v[u] += (float)t[u];
-    } else {
-#pragma unroll
-      for (int u = 0; u < W; u++)
-        if (u < count) v[u] += (float)r[u];
-    }
-  }
-  T* c = (T*)e.c + i * e.ldc + j;
 #pragma unroll
   for (int u = 0; u < W; u++) t[u] = (T)v[u];
-  if constexpr (WIDE) __builtin_memcpy(__builtin_assume_aligned(c, 16), t, sizeof t);
+  if (skip <= 0 && count >= W) __builtin_memcpy(p, t, sizeof t);
   else
 #pragma unroll
     for (int u = 0; u < W; u++)
-      if (u >= skip && u < count) c[u] = t[u];
+      if (u >= skip && u < count) p[u] = t[u];
+}
+template <class T, int W>
+__device__ __forceinline__ void load_row(const T* p, T (&t)[W], int skip, int count) {
+  if (skip <= 0 && count >= W) __builtin_memcpy(t, p, sizeof t);
+  else
+#pragma unroll
+    for (int u = 0; u < W; u++) t[u] = u >= skip && u < count ? p[u] : (T)0.0f;
 }
 
 // Workgroups go to the eight XCDs in turn: each XCD takes one contiguous run of tiles, ordered in bands of eight tile rows with the row running fastest, so
@@ -312,41 +302,79 @@ __device__ __forceinline__ TileAt tile_at(int ti, int tj) {
 }
 
 // Lane l holds column l % 32 and rows 8 (q / 4) + 4 (l / 32) + q % 4 of a 32 x 32 block.  The sums pass through LDS, 32 rows of a wave at a time, so
-// that a lane ends with eight neighbours of one row: whole 16-byte accesses, whole lines.  (Row stride + 8: the two halves of a wave write disjoint banks.)
-// Rows below iown and columns below jown belong to a neighbour.
-template <class T, int MI, int MJ>
-__device__ __forceinline__ void store_tile(const Epilogue& ep, f32x16 (&acc)[MI][MJ], float* stage, int64_t i0, int64_t iown, int64_t iend, int64_t j0, int64_t jown, int64_t jend) {
-  constexpr int W = 8, STRIDE = MJ * 32 + 8, LPR = MJ * 32 / W, RPP = 64 / LPR;
-  const int l = threadIdx.x & 63;
-  const int64_t rows = iend, n = jend;
+// that a lane ends with eight neighbours of one row: 16-byte accesses, whole lines.  (Row stride + 8: the two halves of a wave write disjoint banks.)  A lane
+// keeps its columns, so their bias is loaded once; the residual of 32 rows is on its way while they are staged.  Rows below iown and columns below jown
+// belong to a neighbour.
+template <class T, int ACT, int MI, int MJ>
+__device__ __forceinline__ void store_tile(const Epilogue& ep, f32x16 (&acc)[MI][MJ], float* stage, int64_t i0, int64_t iown, int64_t rows, int64_t j0, int64_t jown, int64_t n) {
+  constexpr int W = 8, STRIDE = MJ * 32 + 8, LPR = MJ * 32 / W, RPP = 64 / LPR, P = 32 / RPP;
+  const int l = threadIdx.x & 63, r0 = l / LPR, col = (l % LPR) * W;
+  const int64_t j = j0 + col;
+  const int count = (int)min((int64_t)W, n - j), skip = (int)min((int64_t)W, jown - j);
+  const bool some = count > 0 && skip < W;
+  float bias[W];
+#pragma unroll
+  for (int u = 0; u < W; u++) bias[u] = 0.0f;
+  if (ep.b && !ep.part && some) {
+    T t[W];
+    load_row<T, W>((const T*)ep.b + j, t, skip, count);
+#pragma unroll
+    for (int u = 0; u < W; u++) bias[u] = (float)t[u];
+  }
 #pragma unroll
   for (int a = 0; a < MI; a++) {
+    T res[P][W];
+    if (ep.r && !ep.part) {
+#pragma unroll
+      for (int p = 0; p < P; p++) {
+        const int64_t i = i0 + a * 32 + p * RPP + r0;
+        if (some && i >= iown && i < rows) load_row<T, W>((const T*)ep.r + i * ep.ldr + j, res[p], skip, count);
+      }
+    }
 #pragma unroll
     for (int b = 0; b < MJ; b++)
 #pragma unroll
       for (int q = 0; q < 16; q++) stage[(8 * (q >> 2) + 4 * (l >> 5) + (q & 3)) * STRIDE + b * 32 + (l & 31)] = acc[a][b][q];
     __builtin_amdgcn_wave_barrier();                             // (a wave's LDS operations happen in order)
-#pragma unroll 1
-    for (int p = 0; p < 32; p += RPP) {
-      const int row = p + l / LPR, col = (l % LPR) * W;
-      const int64_t i = i0 + a * 32 + row, j = j0 + col;
+#pragma unroll
+    for (int p = 0; p < P; p++) {
+      const int row = p * RPP + r0;
+      const int64_t i = i0 + a * 32 + row;
       float v[W];
       __builtin_memcpy(v, __builtin_assume_aligned(stage + row * STRIDE + col, 16), sizeof v);
-      const int count = (int)min((int64_t)W, jend - j), skip = (int)max((int64_t)0, jown - j);
-      if (i >= iown && i < iend && count > 0 && skip < W) {
-        if (ep.part) {
-          float* d = ep.part + ((int64_t)blockIdx.y * rows + i) * n + j;
-          if (ep.wide) __builtin_memcpy(__builtin_assume_aligned(d, 16), v, sizeof v);
-          else
-#pragma unroll
-            for (int u = 0; u < W; u++)
-              if (u >= skip && u < count) d[u] = v[u];
-        } else if (ep.wide) finish<T, W, true>(ep, i, j, n, 0, W, v);
-        else finish<T, W, false>(ep, i, j, n, skip, count, v);
+      if (!some || i < iown || i >= rows) continue;
+      if (ep.part) {
+        store_some<float, W>(ep.part + ((int64_t)blockIdx.y * rows + i) * n + j, v, skip, count);
+        continue;
       }
+#pragma unroll
+      for (int u = 0; u < W; u++) v[u] += bias[u];
+      if (ep.z) store_some<T, W>((T*)ep.z + i * n + j, v, skip, count);
+#pragma unroll
+      for (int u = 0; u < W; u++) v[u] = activate(ACT, v[u]);
+      if (ep.r)
+#pragma unroll
+        for (int u = 0; u < W; u++) v[u] += (float)res[p][u];
+      store_some<T, W>((T*)ep.c + i * ep.ldc + j, v, skip, count);
     }
     __builtin_amdgcn_wave_barrier();
   }
+}
+
+template <class T, bool PLAIN, int MI, int MJ>
+__device__ __forceinline__ void store_tile_any(const Epilogue& ep, f32x16 (&acc)[MI][MJ], float* stage, int64_t i0, int64_t iown, int64_t rows, int64_t j0, int64_t jown, int64_t n) {
+#define MG_ACT(A) store_tile<T, A, MI, MJ>(ep, acc, stage, i0, iown, rows, j0, jown, n)
+  if constexpr (!PLAIN) {
+    switch (ep.part ? MG_ACTIVATION_NONE : ep.act) {
+      case MG_ACTIVATION_RELU: MG_ACT(MG_ACTIVATION_RELU); return;
+      case MG_ACTIVATION_TANH: MG_ACT(MG_ACTIVATION_TANH); return;
+      case MG_ACTIVATION_GELU: MG_ACT(MG_ACTIVATION_GELU); return;
+      case MG_ACTIVATION_SILU: MG_ACT(MG_ACTIVATION_SILU); return;
+      default: break;
+    }
+  }
+  MG_ACT(MG_ACTIVATION_NONE);
+#undef MG_ACT
 }
 
 template <class LA, class LB, int MI, int MJ>
@@ -420,7 +448,7 @@ __global__ __launch_bounds__(WI * WJ * 64) void k_product(Operand A, Operand B, 
   }
   static_assert(WI * WJ * 32 * (MJ * 32 + 8) * 4 <= (int)sizeof lds, "staging fits");
   float* stage = (float*)lds + wave * 32 * (MJ * 32 + 8);
-  store_tile<T, MI, MJ>(ep, acc, stage, i0 + wi, at.i * (int64_t)BI, A.extent, j0 + wj, at.j * (int64_t)BJ, B.extent);
+  store_tile_any<T, BCOLS, MI, MJ>(ep, acc, stage, i0 + wi, at.i * (int64_t)BI, A.extent, j0 + wj, at.j * (int64_t)BJ, B.extent);
 }
 
 template <class T, class SA, class SB, bool ACOLS, bool BCOLS, int BI, int BJ, int WI, int WJ>
@@ -463,7 +491,7 @@ __global__ __launch_bounds__(WI * WJ * 64) void k_product_guarded(Operand A, Ope
   __syncthreads();
   static_assert(WI * WJ * 32 * (MJ * 32 + 8) * 4 <= (int)sizeof lds, "staging fits");
   float* stage = (float*)lds + wave * 32 * (MJ * 32 + 8);
-  store_tile<T, MI, MJ>(ep, acc, stage, i0 + wi, 0, A.extent, j0 + wj, 0, B.extent);
+  store_tile_any<T, BCOLS, MI, MJ>(ep, acc, stage, i0 + wi, 0, A.extent, j0 + wj, 0, B.extent);
 }
 
 // Few rows (a step of a handful of environments): a wave per result column, its lanes along k in chunks of 16 bytes of the weight, one sum per row and lane,
@@ -497,8 +525,7 @@ __global__ __launch_bounds__(256) void k_few_rows(int rows, int64_t k, int64_t n
     mine = lane == i ? s[i] : mine;
   }
   if (lane < rows) {
-    float v[1] = {mine};
-    finish<T, 1, false>(ep, lane, j, n, 0, 1, v);
+    finish<T>(ep, lane, j, n, mine);
   }
 }
 
@@ -528,8 +555,7 @@ __global__ __launch_bounds__(256) void k_join(int64_t total, int64_t n, int spli
     __syncthreads();
     const int64_t at = u0 + threadIdx.x;
     if (at < total) {
-      float v[1] = {(sum[0][threadIdx.x] + sum[1][threadIdx.x]) + (sum[2][threadIdx.x] + sum[3][threadIdx.x])};
-      finish<T, 1, false>(ep, at / n, at % n, n, 0, 1, v);
+      finish<T>(ep, at / n, at % n, n, (sum[0][threadIdx.x] + sum[1][threadIdx.x]) + (sum[2][threadIdx.x] + sum[3][threadIdx.x]));
     }
     __syncthreads();
   }

@@ -27,9 +27,6 @@ static Plan plan_product(int64_t ri, int64_t rj, int64_t depth, int dtype) {
   return p;
 }
 
-// a row stride and an address that allow 16-byte accesses of eight elements of two bytes (of four bytes: twice 16)
-static bool wide_rows(const void* p, int64_t ld) { return ((uintptr_t)p & 15) == 0 && ld % 8 == 0; }
-
 template <class F> static int by_type(int dtype, F f) {
   return dtype == MG_DT_F32 ? f((float*)nullptr) : dtype == MG_DT_BF16 ? f((bf16*)nullptr) : f((f16*)nullptr);
 }
@@ -42,10 +39,7 @@ static int product(hipStream_t st, int form, bool bytes, const Operand& A, const
   if (p.tile >= TILE_64 && std::max(A.ld, B.ld) * TILE_I[p.tile] * 4 >= 0x7fffffffll) p.tile = TILE_GUARDED_128_128;
   if (ceil_div(A.extent, TILE_I[p.tile]) * ceil_div(B.extent, TILE_J[p.tile]) > 0x7fffffffll) return fail(MG_ERR_INVALID, "the result has too many tiles");
   Epilogue first = ep;
-  if (p.splits > 1) {
-    first.part = (float*)ws;
-    first.wide = B.extent % 8 == 0;
-  }
+  if (p.splits > 1) first.part = (float*)ws;
   return by_type(dtype, [&](auto* t) {
     typedef Linear<std::remove_pointer_t<decltype(t)>> L;
     L::product(st, form, bytes, p, A, B, depth, first);
@@ -90,8 +84,7 @@ int mg_op_linear(int device, void* stream, int dtype, int x_dtype, int act, int6
   DeviceGuard g(device);
   if (g.rc != MG_OK) return g.rc;
   hipStream_t st = (hipStream_t)stream;
-  Epilogue ep = {b, r, y, z, nullptr, ldr, ldy, act, 0};
-  ep.wide = n % 8 == 0 && wide_rows(y, ldy) && (!r || wide_rows(r, ldr)) && (!z || wide_rows(z, n));
+  Epilogue ep = {b, r, y, z, nullptr, ldr, ldy, act};
   const bool bytes = x_dtype == MG_DT_U8;
   if (rows <= FEW_ROWS)
     return by_type(dtype, [&](auto* t) {
@@ -136,7 +129,7 @@ int mg_op_linear_dx(int device, void* stream, int dtype, int64_t rows, int64_t k
   if (!dz || !w || !dx || lddz < n || ldw < k) return fail(MG_ERR_INVALID, "dz, w and dx must not be NULL and a row stride not smaller than its row");
   DeviceGuard g(device);
   if (g.rc != MG_OK) return g.rc;
-  Epilogue ep = {nullptr, nullptr, dx, nullptr, nullptr, 0, k, MG_ACTIVATION_NONE, k % 8 == 0 && wide_rows(dx, k)};
+  Epilogue ep = {nullptr, nullptr, dx, nullptr, nullptr, 0, k, MG_ACTIVATION_NONE};
   const Operand A = {dz, lddz, (int32_t)rows}, B = {w, ldw, (int32_t)k};
   return product((hipStream_t)stream, FORM_DX, false, A, B, n, dtype, ep, ws, ws_bytes);
 }
@@ -149,7 +142,7 @@ int mg_op_linear_dw(int device, void* stream, int dtype, int x_dtype, int64_t ro
   if (!dw || (rows && (!dz || !x)) || lddz < n || ldx < k) return fail(MG_ERR_INVALID, "dz, x and dw must not be NULL and a row stride not smaller than its row");
   DeviceGuard g(device);
   if (g.rc != MG_OK) return g.rc;
-  Epilogue ep = {nullptr, nullptr, dw, nullptr, nullptr, 0, k, MG_ACTIVATION_NONE, k % 8 == 0 && wide_rows(dw, k)};
+  Epilogue ep = {nullptr, nullptr, dw, nullptr, nullptr, 0, k, MG_ACTIVATION_NONE};
   const Operand A = {dz, lddz, (int32_t)n}, B = {x, ldx, (int32_t)k};
   return product((hipStream_t)stream, FORM_DW, x_dtype == MG_DT_U8, A, B, rows, dtype, ep, ws, ws_bytes);
 }
