@@ -303,11 +303,12 @@ __device__ __forceinline__ TileAt tile_at(int ti, int tj) {
 
 // Lane l holds column l % 32 and rows 8 (q / 4) + 4 (l / 32) + q % 4 of a 32 x 32 block.  The sums pass through LDS, 32 rows of a wave at a time, so
 // that a lane ends with eight neighbours of one row: 16-byte accesses, whole lines.  (Row stride + 8: the two halves of a wave write disjoint banks.)  A lane
-// keeps its columns, so their bias is loaded once; the residual of 32 rows is on its way while they are staged.  Rows below iown and columns below jown
-// belong to a neighbour.
+// keeps its columns, so their bias is loaded once; its rows go by in groups of G, the residual of the next group on its way while one is finished.  (The
+// groups are a loop: unrolled, an activation's code alone would be larger than the instruction cache.)  Rows below iown and columns below jown belong to
+// a neighbour.
 template <class T, int ACT, int MI, int MJ>
 __device__ __forceinline__ void store_tile(const Epilogue& ep, f32x16 (&acc)[MI][MJ], float* stage, int64_t i0, int64_t iown, int64_t rows, int64_t j0, int64_t jown, int64_t n) {
-  constexpr int W = 8, STRIDE = MJ * 32 + 8, LPR = MJ * 32 / W, RPP = 64 / LPR, P = 32 / RPP;
+  constexpr int W = 8, STRIDE = MJ * 32 + 8, LPR = MJ * 32 / W, RPP = 64 / LPR, P = 32 / RPP, G = P < 2 ? 1 : 2;
   const int l = threadIdx.x & 63, r0 = l / LPR, col = (l % LPR) * W;
   const int64_t j = j0 + col;
   const int count = (int)min((int64_t)W, n - j), skip = (int)min((int64_t)W, jown - j);
@@ -321,41 +322,52 @@ __device__ __forceinline__ void store_tile(const Epilogue& ep, f32x16 (&acc)[MI]
 #pragma unroll
     for (int u = 0; u < W; u++) bias[u] = (float)t[u];
   }
+  const bool residual = ep.r && !ep.part && some;
+  T next[G][W];
+  auto residuals = [&](int p) {                                  // of the group that starts with the p-th of this lane's rows
+    if (residual)
+#pragma unroll
+      for (int u = 0; u < G; u++) {
+        const int64_t i = i0 + (p + u) * RPP + r0;
+        if (i >= iown && i < rows) load_row<T, W>((const T*)ep.r + i * ep.ldr + j, next[u], skip, count);
+      }
+  };
+  residuals(0);
 #pragma unroll
   for (int a = 0; a < MI; a++) {
-    T res[P][W];
-    if (ep.r && !ep.part) {
-#pragma unroll
-      for (int p = 0; p < P; p++) {
-        const int64_t i = i0 + a * 32 + p * RPP + r0;
-        if (some && i >= iown && i < rows) load_row<T, W>((const T*)ep.r + i * ep.ldr + j, res[p], skip, count);
-      }
-    }
 #pragma unroll
     for (int b = 0; b < MJ; b++)
 #pragma unroll
       for (int q = 0; q < 16; q++) stage[(8 * (q >> 2) + 4 * (l >> 5) + (q & 3)) * STRIDE + b * 32 + (l & 31)] = acc[a][b][q];
     __builtin_amdgcn_wave_barrier();                             // (a wave's LDS operations happen in order)
+#pragma unroll 1
+    for (int p = 0; p < P; p += G) {
+      float v[G][W];
+      T res[G][W];
 #pragma unroll
-    for (int p = 0; p < P; p++) {
-      const int row = p * RPP + r0;
-      const int64_t i = i0 + a * 32 + row;
-      float v[W];
-      __builtin_memcpy(v, __builtin_assume_aligned(stage + row * STRIDE + col, 16), sizeof v);
-      if (!some || i < iown || i >= rows) continue;
-      if (ep.part) {
-        store_some<float, W>(ep.part + ((int64_t)blockIdx.y * rows + i) * n + j, v, skip, count);
-        continue;
+      for (int u = 0; u < G; u++) {
+        __builtin_memcpy(v[u], __builtin_assume_aligned(stage + ((p + u) * RPP + r0) * STRIDE + col, 16), sizeof v[u]);
+        __builtin_memcpy(res[u], next[u], sizeof res[u]);
       }
+      if (a * P + p + G < MI * P) residuals(a * P + p + G);
 #pragma unroll
-      for (int u = 0; u < W; u++) v[u] += bias[u];
-      if (ep.z) store_some<T, W>((T*)ep.z + i * n + j, v, skip, count);
+      for (int u = 0; u < G; u++) {
+        const int64_t i = i0 + (a * P + p + u) * RPP + r0;
+        if (!some || i < iown || i >= rows) continue;
+        if (ep.part) {
+          store_some<float, W>(ep.part + ((int64_t)blockIdx.y * rows + i) * n + j, v[u], skip, count);
+          continue;
+        }
 #pragma unroll
-      for (int u = 0; u < W; u++) v[u] = activate(ACT, v[u]);
-      if (ep.r)
+        for (int e = 0; e < W; e++) v[u][e] += bias[e];
+        if (ep.z) store_some<T, W>((T*)ep.z + i * n + j, v[u], skip, count);
 #pragma unroll
-        for (int u = 0; u < W; u++) v[u] += (float)res[p][u];
-      store_some<T, W>((T*)ep.c + i * ep.ldc + j, v, skip, count);
+        for (int e = 0; e < W; e++) v[u][e] = activate(ACT, v[u][e]);
+        if (residual)
+#pragma unroll
+          for (int e = 0; e < W; e++) v[u][e] += (float)res[u][e];
+        store_some<T, W>((T*)ep.c + i * ep.ldc + j, v[u], skip, count);
+      }
     }
     __builtin_amdgcn_wave_barrier();
   }
@@ -447,6 +459,147 @@ __global__ __launch_bounds__(WI * WJ * 64) void k_product(Operand A, Operand B, 
     __syncthreads();
   }
   static_assert(WI * WJ * 32 * (MJ * 32 + 8) * 4 <= (int)sizeof lds, "staging fits");
+  float* stage = (float*)lds + wave * 32 * (MJ * 32 + 8);
+  store_tile_any<T, BCOLS, MI, MJ>(ep, acc, stage, i0 + wi, at.i * (int64_t)BI, A.extent, j0 + wj, at.j * (int64_t)BJ, B.extent);
+}
+
+// An operand's tile from memory straight into LDS, 16 bytes a lane: no registers in between, and nothing waits for it but the wait that is written down.
+// A wave's 64 chunks land one behind the other, so the swizzle is in which chunk a lane asks for.  Needs 16-byte aligned rows and tiles (the host checks).
+template <class T, bool COLS, int EXT, int THREADS>
+struct DirectLoader {
+  typedef Lds<T, COLS, EXT> L;
+  static constexpr int PER = EXT * 8 / THREADS, RPP = THREADS / L::CPR;      // RPP: memory rows per pass of the threads
+  static_assert(sizeof(T) == 2 && EXT == 256 && (!COLS || RPP == 8 || RPP == 16), "the swizzle below");
+  const char* base;            // of the tile that is loaded next
+  int64_t pass, step;
+  uint32_t off[2];             // (cols: bit 3 of a tile row is the parity of the pass where a pass has 8 rows)
+  __device__ __forceinline__ void start(const Operand& o, int i0, int64_t s0) {
+    const int r = (int)threadIdx.x / L::CPR, p = (int)threadIdx.x % L::CPR;
+#pragma unroll
+    for (int q = 0; q < 2; q++) {
+      const int at = COLS ? (p * 16) ^ L::swz(r + q * RPP) : (p ^ (r & 7)) * 16;
+      off[q] = (uint32_t)(r * (int)(o.ld * 2) + at);
+    }
+    pass = (int64_t)RPP * o.ld * 2;
+    step = (COLS ? L::BK * o.ld : L::BK) * 2;
+    base = (const char*)o.p + (COLS ? s0 * o.ld + i0 : (int64_t)i0 * o.ld + s0) * 2;
+  }
+  // pass q of the tile at LDS byte address lds (uniform, like the wave's number)
+  __device__ __forceinline__ void load(int q, uint32_t lds, int wave) {
+    const uint32_t at = lds + q * (THREADS * 16) + wave * 1024;
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(off[COLS ? q & 1 : 0]), "s"(base + q * pass) : "memory");
+  }
+  __device__ __forceinline__ void advance() { base += step; }
+};
+
+// The 256-tile where every row is 16-byte aligned: four waves of 128 x 128, so that a fragment read from LDS feeds four matrix instructions (what a CU reads
+// from LDS takes half as long as what it multiplies; with eight waves of 128 x 64 the two take the same time).  One wave per SIMD: the fragments of a step
+// are read while the step before is multiplied, and the tile after next is on its way to LDS from the moment its buffer is free.  One barrier per tile: it
+// stands where the last fragments of tile t have been read and tile t + 1 has landed.
+template <class T, bool ACOLS, bool BCOLS>
+__global__ __launch_bounds__(256, 1) void k_product_direct(Operand A, Operand B, int64_t depth, int32_t tiles_per_split, Epilogue ep) {
+  constexpr int BI = 256, BJ = 256, THREADS = 256, MI = 4, MJ = 4;
+  typedef DirectLoader<T, ACOLS, BI, THREADS> TA;
+  typedef DirectLoader<T, BCOLS, BJ, THREADS> TB;
+  typedef typename TA::L LA;
+  typedef typename TB::L LB;
+  constexpr int BK = LA::BK, BUF = LA::BYTES + LB::BYTES;
+  __shared__ __attribute__((aligned(1024))) char lds[2 * BUF];
+  const TileAt at = tile_at((A.extent + BI - 1) / BI, (B.extent + BJ - 1) / BJ);
+  const int i0 = min(at.i * BI, A.extent - BI), j0 = min(at.j * BJ, B.extent - BJ);
+  const int64_t first = (int64_t)blockIdx.y * tiles_per_split, last = min((depth + BK - 1) / BK, first + tiles_per_split);
+  const int tiles = (int)(min(depth / BK, last) - first);          // whole tiles; what is left of the axis comes behind them
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wi = (wave >> 1) * 128, wj = (wave & 1) * 128;
+  const uint32_t l0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+
+  f32x16 acc[MI][MJ];
+#pragma unroll
+  for (int a = 0; a < MI; a++)
+#pragma unroll
+    for (int b = 0; b < MJ; b++) acc[a][b] = (f32x16)(0.0f);
+
+  TA ta;
+  TB tb;
+  ta.start(A, i0, first * BK);
+  tb.start(B, j0, first * BK);
+  typename LA::V fa[2][MI];
+  typename LB::V fb[2][MJ];
+  auto read = [&](int s, const char* p, int c, int u) __attribute__((always_inline)) {
+    fa[s][u] = LA::frag(p, wi + u * 32, c);
+    fb[s][u] = LB::frag(p + LA::BYTES, wj + u * 32, c);
+  };
+  // a pass of both operands' next tile, numbered through
+  auto fetch = [&](int q, int t) __attribute__((always_inline)) {
+    const uint32_t p = l0 + (t & 1) * BUF;
+    if (q < TA::PER) ta.load(q, p, wave);
+    else tb.load(q - TA::PER, p + LA::BYTES, wave);
+    if (q == TA::PER - 1) ta.advance();
+    if (q == TA::PER + TB::PER - 1) tb.advance();
+  };
+  constexpr int PASSES = TA::PER + TB::PER, SLOTS = 8;
+  // A step: 16 matrix instructions, four at a time, between them the reads of the next step's fragments and, over two steps, the passes that bring the tile
+  // after next.  Measured at 32 768 x 2048 x 4096 (dx): all passes one behind the other 608 us (the wave waits for the memory pipe to take them), over four
+  // groups 496, over eight 460, over twelve 468 (the last ones land late).
+  auto step = [&](int s, bool reads, const char* p, int c, int slot, bool fetches, int t) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      if (reads) read(s ^ 1, p, c, u);
+      if (fetches && slot >= 0)
+#pragma unroll
+        for (int q = 0; q < PASSES; q++)
+          if (q >= (slot + u) * PASSES / SLOTS && q < (slot + u + 1) * PASSES / SLOTS) fetch(q, t);
+#pragma unroll
+      for (int b = 0; b < MJ; b++) acc[u][b] = mma(fa[s][u], fb[s][b], acc[u][b]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  // tile t; `ahead`: the tile behind it exists; rest / begin: tile t + 1's later passes and tile t + 2's first ones are due
+  auto tile = [&](int t, bool ahead, bool rest, bool begin) __attribute__((always_inline)) {
+    const char* p = lds + (t & 1) * BUF;
+    const char* n = lds + ((t + 1) & 1) * BUF;
+    step(0, true, p, 1, 4, rest, t + 1);
+    step(1, true, p, 2, -1, false, 0);
+    step(0, true, p, 3, -1, false, 0);
+    // (the last fragments are in registers, the next tile has landed, and every wave has come as far)
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    step(1, ahead, n, 0, 0, begin, t + 2);
+  };
+  if (tiles > 0) {
+#pragma unroll
+    for (int q = 0; q < PASSES; q++) fetch(q, 0);
+    if (tiles > 1) {
+#pragma unroll
+      for (int q = 0; q < PASSES / 2; q++) fetch(q, 1);
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PASSES / 2) : "memory");
+    }
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    asm volatile("s_barrier" ::: "memory");
+#pragma unroll
+    for (int u = 0; u < 4; u++) read(0, lds, 0, u);
+    int t = 0;
+    for (; t + 2 < tiles; t++) tile(t, true, true, true);
+    if (t + 1 < tiles) tile(t++, true, true, false);
+    tile(t, false, false, false);
+  }
+  if (first + tiles < last) {                                      // the last piece of the axis, loaded as the last whole one; what was summed is zeroed
+    const int over = (int)(last * BK - depth);
+    Loader<T, T, ACOLS, BI, THREADS> ra;
+    Loader<T, T, BCOLS, BJ, THREADS> rb;
+    ra.start(A, i0, depth - BK);
+    ra.load();
+    ra.store(lds, over);
+    rb.start(B, j0, depth - BK);
+    rb.load();
+    rb.store(lds + LA::BYTES, over);
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+#pragma unroll
+      for (int u = 0; u < 4; u++) read(0, lds, c, u);
+      step(0, false, lds, 0, -1, false, 0);
+    }
+    __syncthreads();
+  }
   float* stage = (float*)lds + wave * 32 * (MJ * 32 + 8);
   store_tile_any<T, BCOLS, MI, MJ>(ep, acc, stage, i0 + wi, at.i * (int64_t)BI, A.extent, j0 + wj, at.j * (int64_t)BJ, B.extent);
 }
@@ -562,13 +715,13 @@ __global__ __launch_bounds__(256) void k_join(int64_t total, int64_t n, int spli
 }
 
 // ---- what mg_linear.hip asks of the translation unit of a type ----
-enum { TILE_GUARDED_32_128, TILE_GUARDED_128_32, TILE_GUARDED_128_128, TILE_64, TILE_128, TILE_256, TILES };
+enum { TILE_GUARDED_32_128, TILE_GUARDED_128_32, TILE_GUARDED_128_128, TILE_64, TILE_128, TILE_256, TILE_DIRECT, TILES };
 enum { FORM_FORWARD, FORM_DX, FORM_DW };          // A rows B rows, A rows B cols, A cols B cols
 struct Plan {
   int tile, splits, per;       // how many ways the summed axis is split, tiles of that axis per split
   int64_t part_bytes;
 };
-constexpr int TILE_I[TILES] = {32, 128, 128, 64, 128, 256}, TILE_J[TILES] = {128, 32, 128, 64, 128, 256};
+constexpr int TILE_I[TILES] = {32, 128, 128, 64, 128, 256, 256}, TILE_J[TILES] = {128, 32, 128, 64, 128, 256, 256};
 constexpr int FEW_ROWS = 8;
 template <class T> struct Linear {
   static void product(hipStream_t st, int form, bool bytes, const Plan& p, const Operand& A, const Operand& B, int64_t depth, const Epilogue& ep);

@@ -37,6 +37,9 @@ static int product(hipStream_t st, int form, bool bytes, const Operand& A, const
   if (p.part_bytes > ws_bytes || (p.part_bytes && (!ws || ((uintptr_t)ws & 255)))) return fail(MG_ERR_INVALID, "workspace: %lld bytes, 256-byte aligned, are needed", (long long)p.part_bytes);
   // (rows so far apart that a tile of them spans 2 GiB: the kernel with 64-bit offsets, same splits)
   if (p.tile >= TILE_64 && std::max(A.ld, B.ld) * TILE_I[p.tile] * 4 >= 0x7fffffffll) p.tile = TILE_GUARDED_128_128;
+  // 16-byte chunks at 16-byte addresses throughout: the operand itself, its rows, and the tiles that were moved back inside
+  auto aligned = [](const Operand& o, bool cols) { return !((uintptr_t)o.p & 15) && o.ld % 8 == 0 && (!cols || o.extent % 8 == 0); };
+  if (p.tile == TILE_256 && dtype != MG_DT_F32 && !bytes && aligned(A, form == FORM_DW) && aligned(B, form != FORM_FORWARD)) p.tile = TILE_DIRECT;
   if (ceil_div(A.extent, TILE_I[p.tile]) * ceil_div(B.extent, TILE_J[p.tile]) > 0x7fffffffll) return fail(MG_ERR_INVALID, "the result has too many tiles");
   Epilogue first = ep;
   if (p.splits > 1) first.part = (float*)ws;

@@ -131,6 +131,28 @@ def test_linear_sizes(size, dt):
     check_linear(x, w, b, r, dy, act, run_linear(x, w, b, r, dy, act))
 
 
+# products large enough for the largest tiles: whole rows of 16 bytes and odd ones, edges that stick out of a tile, and a rest behind the last whole piece of
+# the summed axis, in the forward product and both of the backward pass's (4104, 1032 and 2056 are 8 more than a multiple of 64)
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("size,act,obs", [((4104, 1032, 2056), "gelu", False), ((4096, 1024, 2048), None, False), ((4103, 1031, 2055), "silu", False), ((4104, 1083, 2056), "relu", True)])
+def test_linear_large_tiles(size, act, obs, dt):
+    rows, k, n = size
+    x, w, b, r, dy = linear_inputs(rows, k, n, DT[dt], obs, True, act == "gelu", act == "relu", 11)
+    check_linear(x, w, b, r, dy, act, run_linear(x, w, b, r, dy, act))
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+def test_linear_large_tiles_whatever_the_alignment(dt):
+    """the same numbers from rows at 16-byte addresses and from copies at others"""
+    rows, k, n = 4104, 1032, 2056
+    x, w, b, r, dy = linear_inputs(rows, k, n, DT[dt], False, True, True, False, 12)
+    shift = lambda t, by: torch.nn.functional.pad(t, (by, 16 - by))[:, by:by + t.shape[1]]
+    want = run_linear(x, w, b, r, dy, "silu")
+    for by in (8, 3):
+        got = run_linear(shift(x, by), shift(w, by), b, shift(r, by), shift(dy, by), "silu")
+        assert all(torch.equal(p, q) for p, q in zip(want, got)), by
+
+
 @pytest.mark.parametrize("dt", list(DT))
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("obs", [False, True])
