@@ -39,7 +39,10 @@ static int product(hipStream_t st, int form, bool bytes, const Operand& A, const
   if (p.tile >= TILE_64 && std::max(A.ld, B.ld) * TILE_I[p.tile] * 4 >= 0x7fffffffll) p.tile = TILE_GUARDED_128_128;
   // 16-byte chunks at 16-byte addresses throughout: the operand itself, its rows, and the tiles that were moved back inside
   auto aligned = [](const Operand& o, bool cols) { return !((uintptr_t)o.p & 15) && o.ld % 8 == 0 && (!cols || o.extent % 8 == 0); };
-  if (p.tile == TILE_256 && dtype != MG_DT_F32 && !bytes && aligned(A, form == FORM_DW) && aligned(B, form != FORM_FORWARD)) p.tile = TILE_DIRECT;
+  auto row = [](const void* q, int64_t ld) { return !q || (!((uintptr_t)q & 15) && ld % 8 == 0 && ld < (1 << 22)); };      // (32-bit offsets within a tile)
+  if (p.tile == TILE_256 && dtype != MG_DT_F32 && !bytes && aligned(A, form == FORM_DW) && aligned(B, form != FORM_FORWARD) && B.extent % 8 == 0 && B.extent < (1 << 21) &&
+      row(ep.c, ep.ldc) && row(ep.z, 0) && row(ep.r, ep.ldr) && row(ep.b, 0))
+    p.tile = TILE_DIRECT;
   if (ceil_div(A.extent, TILE_I[p.tile]) * ceil_div(B.extent, TILE_J[p.tile]) > 0x7fffffffll) return fail(MG_ERR_INVALID, "the result has too many tiles");
   Epilogue first = ep;
   if (p.splits > 1) first.part = (float*)ws;
