@@ -55,9 +55,19 @@ MG_API int mg_op_policy_loss_workspace(int64_t rows, int64_t vocab, int64_t* byt
 MG_API int mg_op_policy_loss(int device, void* stream, int dtype, int64_t rows, int64_t vocab, const void* logits, int64_t ld, const void* action, int action_dtype,
                              const float* old_lp, const float* adv, const float* ref_lp, const uint8_t* mask, double clip_lo, double clip_hi, double kl_coef,
                              double ent_coef, float* out, void* save, void* ws, int64_t ws_bytes);
+/* The same, and dlogits (rows, vocab, contiguous; NULL = not wanted) = d loss / d logits along with it.  For rows of more than 64
+ * columns and at most 160 KB: mg_op_policy_loss_makes_gradient says whether (1 or 0). */
+MG_API int mg_op_policy_loss_makes_gradient(int dtype, int64_t vocab);
+MG_API int mg_op_policy_loss_with_gradient(int device, void* stream, int dtype, int64_t rows, int64_t vocab, const void* logits, int64_t ld, const void* action, int action_dtype,
+                                           const float* old_lp, const float* adv, const float* ref_lp, const uint8_t* mask, double clip_lo, double clip_hi, double kl_coef,
+                                           double ent_coef, float* out, void* save, void* ws, int64_t ws_bytes, void* dlogits);
 /* dlogits (rows, vocab, contiguous) = grad[0] * d loss / d logits; rows that do not count get 0 */
 MG_API int mg_op_policy_loss_backward(int device, void* stream, int dtype, int64_t rows, int64_t vocab, const void* logits, int64_t ld, const void* action, int action_dtype,
                                       const uint8_t* mask, double ent_coef, const void* save, const float* grad, void* dlogits);
+
+/* the same for a dlogits that already holds the gradient for the factor 1: left as it is where grad[0] is 1, else computed anew */
+MG_API int mg_op_policy_loss_rescale(int device, void* stream, int dtype, int64_t rows, int64_t vocab, const void* logits, int64_t ld, const void* action, int action_dtype,
+                                     const uint8_t* mask, double ent_coef, const void* save, const float* grad, void* dlogits);
 
 /* ---- one draw per row: action = the lowest k with sum_{j<=k} e^{l_j} > u sum_j e^{l_j}, sums in 64 bits; u NULL: the lowest index of the largest logit ----
  * u (rows, f32 in [0, 1)); action: u8 where vocab <= 256, else i32; lp (rows, f32) = log softmax(logits)[action].  A row without a finite largest logit

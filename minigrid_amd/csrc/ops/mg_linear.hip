@@ -33,15 +33,20 @@ template <class F> static int by_type(int dtype, F f) {
 
 static int product(hipStream_t st, int form, bool bytes, const Operand& A, const Operand& B, int64_t depth, int dtype, Epilogue ep, void* ws, int64_t ws_bytes) {
   if (A.extent == 0 || B.extent == 0) return MG_OK;
+  ep.narrow = std::max({ep.ldc, ep.r ? ep.ldr : 0, (int64_t)B.extent}) < (1 << 21);
   Plan p = plan_product(A.extent, B.extent, depth, dtype);
   if (p.part_bytes > ws_bytes || (p.part_bytes && (!ws || ((uintptr_t)ws & 255)))) return fail(MG_ERR_INVALID, "workspace: %lld bytes, 256-byte aligned, are needed", (long long)p.part_bytes);
   // (rows so far apart that a tile of them spans 2 GiB: the kernel with 64-bit offsets, same splits)
   if (p.tile >= TILE_64 && std::max(A.ld, B.ld) * TILE_I[p.tile] * 4 >= 0x7fffffffll) p.tile = TILE_GUARDED_128_128;
+  // Four waves of 128 x 128 or eight of 128 x 64?  The four multiply faster (65 536 x 1024 x 512: 69 us against 78; 32 768 x 2048 x 4096: 448 against 521),
+  // the eight get a tile's z and residual through faster, which decides up to 512 summed elements (65 536 x 256 x 512 with both: 61 us against 54,
+  // 65 536 x 512 x 512 from cold memory: 99 against 87; 65 536 x 768 x 512: 95 against 102).
+  const bool busy = (ep.z || ep.r) && depth <= 512;
   // 16-byte chunks at 16-byte addresses throughout: the operand itself, its rows, and the tiles that were moved back inside
   auto aligned = [](const Operand& o, bool cols) { return !((uintptr_t)o.p & 15) && o.ld % 8 == 0 && (!cols || o.extent % 8 == 0); };
-  auto row = [](const void* q, int64_t ld) { return !q || (!((uintptr_t)q & 15) && ld % 8 == 0 && ld < (1 << 22)); };      // (32-bit offsets within a tile)
-  if (p.tile == TILE_256 && dtype != MG_DT_F32 && !bytes && aligned(A, form == FORM_DW) && aligned(B, form != FORM_FORWARD) && B.extent % 8 == 0 && B.extent < (1 << 21) &&
-      row(ep.c, ep.ldc) && row(ep.z, 0) && row(ep.r, ep.ldr) && row(ep.b, 0))
+  auto row = [](const void* q, int64_t ld) { return !q || (!((uintptr_t)q & 15) && ld % 8 == 0); };
+  if (p.tile == TILE_256 && dtype != MG_DT_F32 && !bytes && aligned(A, form == FORM_DW) && aligned(B, form != FORM_FORWARD) && B.extent % 8 == 0 && ep.narrow &&
+      row(ep.c, ep.ldc) && row(ep.z, 0) && row(ep.r, ep.ldr) && row(ep.b, 0) && !busy)
     p.tile = TILE_DIRECT;
   if (ceil_div(A.extent, TILE_I[p.tile]) * ceil_div(B.extent, TILE_J[p.tile]) > 0x7fffffffll) return fail(MG_ERR_INVALID, "the result has too many tiles");
   Epilogue first = ep;
@@ -90,7 +95,7 @@ int mg_op_linear(int device, void* stream, int dtype, int x_dtype, int act, int6
   DeviceGuard g(device);
   if (g.rc != MG_OK) return g.rc;
   hipStream_t st = (hipStream_t)stream;
-  Epilogue ep = {b, r, y, z, nullptr, ldr, ldy, act};
+  Epilogue ep = {b, r, y, z, nullptr, ldr, ldy, act, 0};
   const bool bytes = x_dtype == MG_DT_U8;
   if (rows <= FEW_ROWS)
     return by_type(dtype, [&](auto* t) {
@@ -135,7 +140,7 @@ int mg_op_linear_dx(int device, void* stream, int dtype, int64_t rows, int64_t k
   if (!dz || !w || !dx || lddz < n || ldw < k) return fail(MG_ERR_INVALID, "dz, w and dx must not be NULL and a row stride not smaller than its row");
   DeviceGuard g(device);
   if (g.rc != MG_OK) return g.rc;
-  Epilogue ep = {nullptr, nullptr, dx, nullptr, nullptr, 0, k, MG_ACTIVATION_NONE};
+  Epilogue ep = {nullptr, nullptr, dx, nullptr, nullptr, 0, k, MG_ACTIVATION_NONE, 0};
   const Operand A = {dz, lddz, (int32_t)rows}, B = {w, ldw, (int32_t)k};
   return product((hipStream_t)stream, FORM_DX, false, A, B, n, dtype, ep, ws, ws_bytes);
 }
@@ -148,7 +153,7 @@ int mg_op_linear_dw(int device, void* stream, int dtype, int x_dtype, int64_t ro
   if (!dw || (rows && (!dz || !x)) || lddz < n || ldx < k) return fail(MG_ERR_INVALID, "dz, x and dw must not be NULL and a row stride not smaller than its row");
   DeviceGuard g(device);
   if (g.rc != MG_OK) return g.rc;
-  Epilogue ep = {nullptr, nullptr, dw, nullptr, nullptr, 0, k, MG_ACTIVATION_NONE};
+  Epilogue ep = {nullptr, nullptr, dw, nullptr, nullptr, 0, k, MG_ACTIVATION_NONE, 0};
   const Operand A = {dz, lddz, (int32_t)n}, B = {x, ldx, (int32_t)k};
   return product((hipStream_t)stream, FORM_DW, x_dtype == MG_DT_U8, A, B, rows, dtype, ep, ws, ws_bytes);
 }

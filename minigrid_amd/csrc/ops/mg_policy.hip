@@ -50,7 +50,7 @@ template <class A> __device__ __forceinline__ int64_t action_of(const A& a, int6
 struct Terms { double policy, kl, entropy, clipped, count; };
 
 // the loss terms of a row that counts, from its statistics
-__device__ __forceinline__ void row_terms(const LossArgs& a, int64_t i, double lse, double entropy, double chosen, Terms& sum) {
+__device__ __forceinline__ Saved row_terms(const LossArgs& a, int64_t i, double lse, double entropy, double chosen, Terms& sum) {
   const double lp = chosen - lse, adv = a.adv[i], q = exp(lp - (double)a.old_lp[i]);
   const bool clipped = adv >= 0.0 ? q > a.hi : q < a.lo;
   const double policy = -(clipped ? (adv >= 0.0 ? a.hi : a.lo) : q) * adv;
@@ -60,8 +60,10 @@ __device__ __forceinline__ void row_terms(const LossArgs& a, int64_t i, double l
     kl = e - gap - 1.0;
     dlp += a.kl * (1.0 - e);
   }
-  if (a.save) a.save[i] = {lse, (float)dlp, (float)entropy};
+  const Saved k = {lse, (float)dlp, (float)entropy};
+  if (a.save) a.save[i] = k;
   sum.policy += policy; sum.kl += kl; sum.entropy += entropy; sum.clipped += clipped ? 1.0 : 0.0; sum.count += 1.0;
+  return k;
 }
 
 __device__ __forceinline__ void write_out(const LossArgs& a, const Terms& t, float* out) {
@@ -149,15 +151,6 @@ __global__ void k_loss_small(LossArgs a, double* part, float* out) {
 // ---- long rows ----
 struct Sums { float m; double s, t; };
 
-__device__ __forceinline__ void join(Sums& a, float m, double s, double t) {      // a += (m, s, t)
-  const float M = fmaxf(a.m, m);
-  const double da = a.m == NEG_INF ? 0.0 : (double)a.m - (double)M, db = m == NEG_INF ? 0.0 : (double)m - (double)M;      // (a part without a finite logit has s = t = 0)
-  const double fa = exp_neg(da), fb = exp_neg(db);
-  a.t = fa * (a.t + da * a.s) + fb * (t + db * s);
-  a.s = fa * a.s + fb * s;
-  a.m = M;
-}
-
 template <int N>
 __device__ __forceinline__ void add_chunk(Sums& a, const float (&x)[N]) {
   float top = x[0];
@@ -234,28 +227,6 @@ __device__ __forceinline__ void wave_join(Sums& a) {
   a.m = M;
 }
 
-// a workgroup per row
-template <class T>
-__global__ __launch_bounds__(256) void k_loss_rows(LossArgs a, double* part) {
-  __shared__ Sums w[4];
-  const int64_t i = blockIdx.x;
-  Terms sum = {};
-  if (!a.mask || a.mask[i]) {                                    // (uniform in the workgroup)
-    const T* row = (const T*)a.logits + i * a.ld;
-    Sums s = row_sums<T, 256>(row, 0, a.vocab, threadIdx.x);
-    wave_join(s);
-    if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = s;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      for (int v = 1; v < 4; v++) join(s, w[v].m, w[v].s, w[v].t);
-      const double ls = log(s.s);
-      const int64_t act = action_of(a, i);
-      row_terms(a, i, (double)s.m + ls, ls - s.t / s.s, act >= 0 && act < a.vocab ? (double)(float)row[act] : __builtin_nan(""), sum);
-    }
-  }
-  if (threadIdx.x == 0) put_part(part, a.rows, i, sum);
-}
-
 // d loss / d logit_j = g / count (dlp (1[j = action] - p_j) + ent p_j (l_j - lse + H)), p_j = e^{l_j - lse}
 struct GradArgs {
   const void* logits; int64_t ld; const void* action; int32_t action_dtype; const uint8_t* mask;
@@ -297,39 +268,243 @@ __global__ void k_grad_small(GradArgs a) {
   }
 }
 
-constexpr int64_t GRAD_RUN = 16384;      // elements of a row per workgroup
-
-template <class T>
-__global__ __launch_bounds__(256) void k_grad_rows(GradArgs a) {
-  constexpr int N = Pack<T>::N;
-  // (the last rows first: the forward pass has just left them in the cache behind the L2s)
-  const int64_t i = a.rows - 1 - (int64_t)blockIdx.x, from = (int64_t)blockIdx.y * GRAD_RUN, to = min(a.vocab, from + GRAD_RUN);
-  const bool on = !a.mask || a.mask[i];
-  const T* row = (const T*)a.logits + i * a.ld;
-  T* d = (T*)a.dlogits + i * a.vocab;
-  Saved s = {0.0, 0.0f, 0.0f};
-  float dlp = 0.0f, ent = 0.0f;
-  int64_t act = -1;
-  if (on) {
-    s = a.save[i];
-    const float share = a.grad[0] / (float)a.save[a.rows].lse;
-    dlp = s.dlp * share; ent = a.ent * share; act = action_of(a, i);
+// The gradient of a long row, in powers of two: with y = (l - lse) log2 e it is 2^y (ent ln 2 (y + H log2 e) - dlp), plus dlp at the action.  lse comes in
+// two parts: l - hi is as good as exact where p is large.
+struct GradRow {
+  float hi, lo2, ent2, k, dlp;
+  __device__ __forceinline__ GradRow(const Saved& s, float dlp_, float ent) : hi((float)s.lse), ent2(ent * (float)LN2), dlp(dlp_) {
+    lo2 = (float)(s.lse - (double)hi) * LOG2E_HI;
+    k = __builtin_fmaf(ent, s.entropy, -dlp_);
   }
+  __device__ __forceinline__ float operator()(float l) const {
+    const float y = __builtin_fmaf(l - hi, LOG2E_HI, -lo2);
+    return __builtin_amdgcn_exp2f(y) * __builtin_fmaf(ent2, fmaxf(y, -300.0f), k);           // (a NaN is in the first factor, and a closed column's is 0)
+  }
+  // the chunk of columns c..c + N
+  template <class T, int N> __device__ __forceinline__ void chunk(T* x, int64_t c, int64_t act) const {
+    float g[N];
+#pragma unroll
+    for (int u = 0; u < N; u++) g[u] = (*this)((float)x[u]);
+    if ((uint64_t)(act - c) < N)                                 // (rarely: no lane of the wave has it)
+#pragma unroll
+      for (int u = 0; u < N; u++) g[u] += c + u == act ? dlp : 0.0f;
+#pragma unroll
+    for (int u = 0; u < N; u++) x[u] = (T)g[u];
+  }
+};
+
+// the gradient of elements [from, to) of a row that counts, or zeros
+template <class T, int NT>
+__device__ __forceinline__ void grad_run(const T* row, T* d, int64_t from, int64_t to, bool on, const GradRow& g, int64_t act) {
+  constexpr int N = Pack<T>::N;
   // whole 16-byte stores: the run is counted from the gradient's alignment, the logits may lie at any
   const int64_t skew = (int64_t)(((uintptr_t)(d + from) & 15) / sizeof(T));
   const int64_t head = min(to, from + (skew ? N - skew : 0)), body = head + (to - head) / N * N;
-  auto one = [&](int64_t c) { d[c] = on ? (T)grad_of((float)row[c], s.lse, s.entropy, dlp, ent, c == act) : (T)0.0f; };
+  auto one = [&](int64_t c) {
+    T x[1] = {(T)0.0f};
+    if (on) {
+      x[0] = row[c];
+      g.chunk<T, 1>(x, c, act);
+    }
+    d[c] = x[0];
+  };
   if (from + threadIdx.x < head) one(from + threadIdx.x);
-  for (int64_t c = head + (int64_t)threadIdx.x * N; c < body; c += 256 * N) {
+#pragma unroll 2
+  for (int64_t c = head + (int64_t)threadIdx.x * N; c < body; c += NT * N) {
     T v[N] = {};
     if (on) {
       __builtin_memcpy(v, row + c, 16);
-#pragma unroll
-      for (int u = 0; u < N; u++) v[u] = (T)grad_of((float)v[u], s.lse, s.entropy, dlp, ent, c + u == act);
+      g.chunk<T, N>(v, c, act);
     }
     __builtin_memcpy(__builtin_assume_aligned(d + c, 16), v, 16);
   }
   if (body + threadIdx.x < to) one(body + threadIdx.x);
+}
+
+// how many rows count: one workgroup
+__global__ __launch_bounds__(1024) void k_count(const uint8_t* mask, int64_t rows, double* count) {
+  __shared__ int64_t w[16];
+  int64_t n = 0;
+#pragma unroll 4
+  for (int64_t i = threadIdx.x; i < rows; i += 1024) n += mask[i] ? 1 : 0;
+#pragma unroll
+  for (int m = 32; m; m >>= 1) n += __shfl_xor((int)n, m);       // (a lane has less than 2^21 of them)
+  if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = n;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    n = 0;
+    for (int v = 0; v < 16; v++) n += w[v];
+    *count = (double)n;
+  }
+}
+
+// what a row's thread 0 makes of its sums
+template <class T>
+__device__ __forceinline__ Saved row_result(const LossArgs& a, int64_t i, const T* row, float m, double s, double t, Terms& sum) {
+  const double ls = log(s);
+  const int64_t act = action_of(a, i);
+  return row_terms(a, i, (double)m + ls, ls - t / s, act >= 0 && act < a.vocab ? (double)(float)row[act] : __builtin_nan(""), sum);
+}
+
+// (called, not inlined: the constants of its exp and log would be held in registers over the whole loop, next to the row)
+template <class T>
+__device__ __noinline__ Saved row_result_call(const LossArgs& a, int64_t i, const T* row, float m, double s, double t, Terms* sum) { return row_result(a, i, row, m, s, t, *sum); }
+
+// A workgroup per row at a time, every gridDim-th row: rows of up to C x NT 16-byte chunks are held in registers, so the maximum, the sums and, where
+// dlogits is wanted, the gradient (for the factor 1) take one trip to memory.  16 384 x 40 961 bf16, a quarter masked: 2.35 GB in 625 us, 3.8 TB/s, bound by
+// memory and by about twenty vector instructions an element together (two workgroups a CU, 124 registers).  The loss and the gradient from two readings
+// took 719 us, a second reading through the caches 814.
+// count: how many rows count (where dlogits and a mask are there), else all do.
+template <class T, int NT, int C>
+__global__ __launch_bounds__(NT, 4) void k_loss_held(LossArgs a, double* part, const double* count, T* dlogits) {
+  constexpr int N = Pack<T>::N, W = NT / 64;
+  typedef T VT __attribute__((ext_vector_type(N)));
+  __shared__ float wm[W];
+  __shared__ double ws[W], wt[W];
+  __shared__ Saved saved;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  Terms sum = {};
+  float share = 0.0f;
+  if (dlogits) share = 1.0f / (float)(a.mask ? *count : (double)a.rows);
+  for (int64_t i = blockIdx.x; i < a.rows; i += gridDim.x) {
+    const T* row = (const T*)a.logits + i * a.ld;
+    T* d = dlogits + i * a.vocab;
+    // whole 16-byte chunks as the gradient's alignment deals them (the logits may lie at any); in front of and behind them less than a chunk
+    const int skew = dlogits ? (int)(((uintptr_t)d & 15) / sizeof(T)) : (int)(((uintptr_t)(i * a.vocab * sizeof(T)) & 15) / sizeof(T));
+    const int vocab = (int)a.vocab, head = min(vocab, skew ? N - skew : 0), body = head + (vocab - head) / N * N;
+    if (a.mask && !a.mask[i]) {                                  // (uniform in the workgroup)
+      if (dlogits) {
+        if (tid < head) d[tid] = (T)0.0f;
+        for (int c = head + tid * N; c < body; c += NT * N) *(u32x4*)__builtin_assume_aligned(d + c, 16) = (u32x4)(0u);
+        if (body + tid < vocab) d[body + tid] = (T)0.0f;
+      }
+      continue;
+    }
+    u32x4 v[C];
+    T edge = (T)NEG_INF;
+    // the chunk's elements, widened where they are used: otherwise they would be kept widened, and not fit
+    auto chunk = [&](int q) __attribute__((always_inline)) {
+      asm volatile("" : "+v"(v[q]));
+      return __builtin_bit_cast(VT, v[q]);
+    };
+    const int at = tid < head ? tid : tid >= 64 && body + tid - 64 < vocab ? body + tid - 64 : -1;      // an element of the head, or of the rest
+#pragma unroll
+    for (int q = 0; q < C; q++) {
+      const int c = head + (q * NT + tid) * N;
+      v[q] = (u32x4)(sizeof(T) == 4 ? 0xff800000u : std::is_same_v<T, bf16> ? 0xff80ff80u : 0xfc00fc00u);        // -inf
+      if (c < body) __builtin_memcpy(&v[q], row + c, 16);
+    }
+    if (at >= 0) edge = row[at];
+    float m = (float)edge;
+#pragma unroll
+    for (int q = 0; q < C; q++) {
+      const VT x = chunk(q);
+#pragma unroll
+      for (int u = 0; u < N; u++) m = fmaxf(m, (float)x[u]);
+    }
+    m = wave_max(m);
+    if (lane == 0) wm[wave] = m;
+    __syncthreads();
+    m = wm[0];
+#pragma unroll
+    for (int w = 1; w < W; w++) m = fmaxf(m, wm[w]);
+    double s = 0.0, t = 0.0;
+    auto add = [&](float x, float& e8, float& t8) __attribute__((always_inline)) {
+      const float z = (x - m) * LOG2E_HI, e = __builtin_amdgcn_exp2f(z);
+      e8 += e;
+      t8 = __builtin_fmaf(e, fmaxf(z, -300.0f), t8);             // (2^-300 is 0 in 32 bits; a NaN is in e)
+    };
+#pragma unroll
+    for (int q = 0; q < C; q++) {
+      if (head + (q * NT + (tid & ~63)) * N >= body) break;      // (uniform in the wave)
+      const VT x = chunk(q);
+      float e8 = 0.0f, t8 = 0.0f;                                // at most eight terms in 32 bits, then into the 64-bit sum
+#pragma unroll
+      for (int u = 0; u < N; u++) add((float)x[u], e8, t8);
+      s += (double)e8;
+      t += (double)t8;
+    }
+    {
+      float e8 = 0.0f, t8 = 0.0f;
+      if (at >= 0) add((float)edge, e8, t8);
+      s += (double)e8;
+      t += (double)t8;
+    }
+    s = wave_sum(s);
+    t = wave_sum(t);
+    if (lane == 0) { ws[wave] = s; wt[wave] = t; }
+    __syncthreads();
+    if (tid == 0) {
+#pragma unroll
+      for (int w = 1; w < W; w++) { s += ws[w]; t += wt[w]; }
+      saved = row_result_call<T>(a, i, row, m, s, t * LN2, &sum);
+    }
+    if (!dlogits) continue;                                      // (thread 0 has read what the next row overwrites before it comes to the next barrier)
+    __syncthreads();
+    const GradRow g(saved, saved.dlp * share, (float)a.ent * share);
+    const int act = (int)min((int64_t)0x7fffffff, max((int64_t)-1, action_of(a, i)));
+#pragma unroll
+    for (int q = 0; q < C; q++) {
+      const int c = head + (q * NT + tid) * N;
+      if (c < body) {
+        T x[N];
+        const VT h = chunk(q);
+        __builtin_memcpy(x, &h, sizeof x);
+        g.chunk<T, N>(x, c, act);
+        __builtin_memcpy(__builtin_assume_aligned(d + c, 16), x, 16);
+      }
+    }
+    if (at >= 0) {
+      T x[1] = {edge};
+      g.chunk<T, 1>(x, at, act);
+      d[at] = x[0];
+    }
+  }
+  if (tid == 0) put_part(part, gridDim.x, blockIdx.x, sum);
+}
+
+// rows that no workgroup's registers hold: their sums alone, the maximum running along
+template <class T>
+__global__ __launch_bounds__(256, 4) void k_loss_rows(LossArgs a, double* part) {
+  __shared__ Sums w[4];
+  Terms sum = {};
+  for (int64_t i = blockIdx.x; i < a.rows; i += gridDim.x) {
+    if (a.mask && !a.mask[i]) continue;                          // (uniform in the workgroup)
+    const T* row = (const T*)a.logits + i * a.ld;
+    Sums s = row_sums<T, 256>(row, 0, a.vocab, threadIdx.x);
+    wave_join(s);
+    __syncthreads();                                             // (the row before is done with w)
+    if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x < 64) {
+      s = threadIdx.x < 4 ? w[threadIdx.x] : Sums{NEG_INF, 0.0, 0.0};
+      wave_join(s);
+      if (threadIdx.x == 0) row_result(a, i, row, s.m, s.s, s.t, sum);
+    }
+  }
+  if (threadIdx.x == 0) put_part(part, gridDim.x, blockIdx.x, sum);
+}
+
+constexpr int64_t GRAD_RUN = 16384;      // elements of a row per workgroup at a time
+
+// unless_one: nothing is to be done for the factor 1
+template <class T>
+__global__ __launch_bounds__(256) void k_grad_rows(GradArgs a, int64_t runs, int unless_one) {
+  if (unless_one && a.grad[0] == 1.0f) return;
+  for (int64_t u = blockIdx.x; u < a.rows * runs; u += gridDim.x) {
+    // (the last rows first: the forward pass has just left them in the cache behind the L2s)
+    const int64_t i = a.rows - 1 - u / runs, from = u % runs * GRAD_RUN, to = min(a.vocab, from + GRAD_RUN);
+    const bool on = !a.mask || a.mask[i];
+    Saved s = {0.0, 0.0f, 0.0f};
+    float dlp = 0.0f, ent = 0.0f;
+    int64_t act = -1;
+    if (on) {
+      s = a.save[i];
+      const float share = a.grad[0] / (float)a.save[a.rows].lse;
+      dlp = s.dlp * share; ent = a.ent * share; act = action_of(a, i);
+    }
+    grad_run<T, 256>((const T*)a.logits + i * a.ld, (T*)a.dlogits + i * a.vocab, from, to, on, GradRow(s, dlp, ent), act);
+  }
 }
 
 // ---- the draw ----
@@ -541,6 +716,14 @@ template <class F> static int by_type(int dtype, F f) {
   return dtype == MG_DT_F32 ? f((const float*)nullptr) : dtype == MG_DT_BF16 ? f((const bf16*)nullptr) : f((const f16*)nullptr);
 }
 
+// workgroups of the loss over its rows: for long rows at most 4096, each with its share of them
+static int64_t loss_groups(int64_t rows, int64_t vocab) {
+  if (vocab <= SMALL_VOCAB) return (rows + small_rows(vocab) - 1) / small_rows(vocab);
+  const int64_t per = (rows + 4095) / 4096;
+  return per ? (rows + per - 1) / per : 0;
+}
+constexpr int64_t HELD_BYTES = 160 * 1024;  // the longest row that a workgroup's registers hold
+
 static size_t small_lds(int R, int64_t vocab) { return std::max<size_t>((size_t)R * (vocab | 1) * 4, 4 * sizeof(Terms)); }
 
 }  // namespace mgo
@@ -552,28 +735,31 @@ extern "C" {
 int mg_op_policy_loss_workspace(int64_t rows, int64_t vocab, int64_t* bytes) {
   const int rc = check_logits(MG_DT_F32, rows, vocab, vocab);
   if (rc != MG_OK) return rc;
-  *bytes = (vocab <= SMALL_VOCAB ? (rows + small_rows(vocab) - 1) / small_rows(vocab) : rows) * (int64_t)sizeof(Terms);
+  if (!bytes) return fail(MG_ERR_INVALID, "bytes must not be NULL");
+  *bytes = loss_groups(rows, vocab) * (int64_t)sizeof(Terms) + 16;          // (behind the sums: the number of rows that count)
   return MG_OK;
 }
 
-int mg_op_policy_loss(int device, void* stream, int dtype, int64_t rows, int64_t vocab, const void* logits, int64_t ld, const void* action, int action_dtype, const float* old_lp,
-                      const float* adv, const float* ref_lp, const uint8_t* mask, double clip_lo, double clip_hi, double kl_coef, double ent_coef, float* out,
-                      void* save, void* ws, int64_t ws_bytes) {
+int mg_op_policy_loss_makes_gradient(int dtype, int64_t vocab) { return vocab > SMALL_VOCAB && vocab * dtype_bytes(dtype) <= HELD_BYTES; }
+
+int mg_op_policy_loss_with_gradient(int device, void* stream, int dtype, int64_t rows, int64_t vocab, const void* logits, int64_t ld, const void* action, int action_dtype,
+                                    const float* old_lp, const float* adv, const float* ref_lp, const uint8_t* mask, double clip_lo, double clip_hi, double kl_coef,
+                                    double ent_coef, float* out, void* save, void* ws, int64_t ws_bytes, void* dlogits) {
   int rc = check_logits(dtype, rows, vocab, ld);
   if (rc == MG_OK) rc = check_action(action_dtype);
   if (rc != MG_OK) return rc;
   if (!out || (rows && (!logits || !action || !old_lp || !adv))) return fail(MG_ERR_INVALID, "logits, action, old_lp, adv and out must not be NULL");
+  if (dlogits && !mg_op_policy_loss_makes_gradient(dtype, vocab)) return fail(MG_ERR_INVALID, "no gradient comes with the loss for rows of this length");
   int64_t need = 0;
   mg_op_policy_loss_workspace(rows, vocab, &need);
-  if (ws_bytes < need || (need && (!ws || ((uintptr_t)ws & 15)))) return fail(MG_ERR_INVALID, "workspace: %lld bytes are needed", (long long)need);
+  if (ws_bytes < need || !ws || ((uintptr_t)ws & 15)) return fail(MG_ERR_INVALID, "workspace: %lld bytes are needed", (long long)need);
   DeviceGuard g(device);
   if (g.rc != MG_OK) return g.rc;
   hipStream_t st = (hipStream_t)stream;
   LossArgs a = {logits, ld, action, action_dtype, old_lp, adv, ref_lp, mask, 1.0 - clip_lo, 1.0 + clip_hi, kl_coef, ent_coef, (Saved*)save, rows, vocab};
-  int64_t parts = 0;
+  const int64_t parts = loss_groups(rows, vocab);
   if (rows && vocab <= SMALL_VOCAB) {
     const int R = small_rows(vocab);
-    parts = (rows + R - 1) / R;
     by_type(dtype, [&](auto* t) {
       typedef std::remove_cv_t<std::remove_pointer_t<decltype(t)>> T;
       k_loss_small<T><<<(unsigned)parts, R, small_lds(R, vocab), st>>>(a, (double*)ws, out);
@@ -581,10 +767,18 @@ int mg_op_policy_loss(int device, void* stream, int dtype, int64_t rows, int64_t
     });
     if (parts == 1) return launched("policy loss");
   } else if (rows) {
-    parts = rows;
+    double* count = (double*)ws + parts * 5;
+    if (dlogits && mask) k_count<<<1, 1024, 0, st>>>(mask, rows, count);
     by_type(dtype, [&](auto* t) {
       typedef std::remove_cv_t<std::remove_pointer_t<decltype(t)>> T;
-      k_loss_rows<T><<<(unsigned)rows, 256, 0, st>>>(a, (double*)ws);
+      const int64_t bytes = vocab * (int64_t)sizeof(T), kb = 1024;
+#define MG_HELD(NT, C) k_loss_held<T, NT, C><<<(unsigned)parts, NT, 0, st>>>(a, (double*)ws, count, (T*)dlogits)
+      if (bytes <= 16 * kb) MG_HELD(256, 4);
+      else if (bytes <= 32 * kb) MG_HELD(512, 4);
+      else if (bytes <= 80 * kb + 15) MG_HELD(512, 10);          // (a row of up to 15 bytes more has no chunk more: they are not whole)
+      else if (bytes <= HELD_BYTES) MG_HELD(1024, 10);
+      else k_loss_rows<T><<<(unsigned)parts, 256, 0, st>>>(a, (double*)ws);
+#undef MG_HELD
       return 0;
     });
   }
@@ -592,12 +786,20 @@ int mg_op_policy_loss(int device, void* stream, int dtype, int64_t rows, int64_t
   return launched("policy loss");
 }
 
-int mg_op_policy_loss_backward(int device, void* stream, int dtype, int64_t rows, int64_t vocab, const void* logits, int64_t ld, const void* action, int action_dtype,
-                               const uint8_t* mask, double ent_coef, const void* save, const float* grad, void* dlogits) {
+int mg_op_policy_loss(int device, void* stream, int dtype, int64_t rows, int64_t vocab, const void* logits, int64_t ld, const void* action, int action_dtype, const float* old_lp,
+                      const float* adv, const float* ref_lp, const uint8_t* mask, double clip_lo, double clip_hi, double kl_coef, double ent_coef, float* out,
+                      void* save, void* ws, int64_t ws_bytes) {
+  return mg_op_policy_loss_with_gradient(device, stream, dtype, rows, vocab, logits, ld, action, action_dtype, old_lp, adv, ref_lp, mask, clip_lo, clip_hi, kl_coef, ent_coef, out,
+                                         save, ws, ws_bytes, nullptr);
+}
+
+static int loss_backward(int device, void* stream, int dtype, int64_t rows, int64_t vocab, const void* logits, int64_t ld, const void* action, int action_dtype, const uint8_t* mask,
+                         double ent_coef, const void* save, const float* grad, void* dlogits, bool unless_one) {
   int rc = check_logits(dtype, rows, vocab, ld);
   if (rc == MG_OK) rc = check_action(action_dtype);
   if (rc != MG_OK || rows == 0) return rc;
   if (!logits || !action || !save || !grad || !dlogits) return fail(MG_ERR_INVALID, "no pointer but mask may be NULL");
+  if (unless_one && !mg_op_policy_loss_makes_gradient(dtype, vocab)) return fail(MG_ERR_INVALID, "no gradient comes with the loss for rows of this length");
   DeviceGuard g(device);
   if (g.rc != MG_OK) return g.rc;
   hipStream_t st = (hipStream_t)stream;
@@ -609,11 +811,20 @@ int mg_op_policy_loss_backward(int device, void* stream, int dtype, int64_t rows
       k_grad_small<T><<<(unsigned)((rows + R - 1) / R), R, small_lds(R, vocab), st>>>(a);
     } else {
       const int64_t runs = (vocab + GRAD_RUN - 1) / GRAD_RUN;
-      if (runs > 65535) return fail(MG_ERR_INVALID, "vocab above 2^30 is not supported");
-      k_grad_rows<T><<<dim3((unsigned)rows, (unsigned)runs), 256, 0, st>>>(a);
+      k_grad_rows<T><<<(unsigned)std::min<int64_t>(rows * runs, unless_one ? 2048 : 1 << 20), 256, 0, st>>>(a, runs, unless_one);
     }
     return launched("policy loss backward");
   });
+}
+
+int mg_op_policy_loss_backward(int device, void* stream, int dtype, int64_t rows, int64_t vocab, const void* logits, int64_t ld, const void* action, int action_dtype,
+                               const uint8_t* mask, double ent_coef, const void* save, const float* grad, void* dlogits) {
+  return loss_backward(device, stream, dtype, rows, vocab, logits, ld, action, action_dtype, mask, ent_coef, save, grad, dlogits, false);
+}
+
+int mg_op_policy_loss_rescale(int device, void* stream, int dtype, int64_t rows, int64_t vocab, const void* logits, int64_t ld, const void* action, int action_dtype,
+                              const uint8_t* mask, double ent_coef, const void* save, const float* grad, void* dlogits) {
+  return loss_backward(device, stream, dtype, rows, vocab, logits, ld, action, action_dtype, mask, ent_coef, save, grad, dlogits, true);
 }
 
 int mg_op_sample_workspace(int64_t rows, int64_t vocab, int64_t* bytes) {

@@ -24,7 +24,7 @@ typedef std::optional<Tensor> MaybeTensor;
 
 #define MG_ENTRIES(X) \
   X(mg_ops_last_error) X(mg_op_linear_workspace) X(mg_op_linear) X(mg_op_linear_dz_workspace) X(mg_op_linear_dz) X(mg_op_linear_dx) X(mg_op_linear_dw) \
-  X(mg_op_policy_loss_workspace) X(mg_op_policy_loss) X(mg_op_policy_loss_backward) X(mg_op_sample_workspace) X(mg_op_sample) X(mg_op_advantages)
+  X(mg_op_policy_loss_workspace) X(mg_op_policy_loss) X(mg_op_policy_loss_makes_gradient) X(mg_op_policy_loss_with_gradient) X(mg_op_policy_loss_backward) X(mg_op_policy_loss_rescale) X(mg_op_sample_workspace) X(mg_op_sample) X(mg_op_advantages)
 struct Entries {
 #define X(name) decltype(&::name) name = nullptr;
   MG_ENTRIES(X)
@@ -122,10 +122,12 @@ variable_list no_second(const char* name, variable_list&& grads, std::initialize
   return std::move(grads);
 }
 
+bool capturing() { return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None; }
+
 // A captured step must not meet an eager graph of the same leaves that is still alive: the leaves' gradient nodes belong to the stream that graph was recorded
 // on, the backward pass would wait on that stream from inside the capture, and torch ends the process there.  Said here, where it can still be said.
 void refuse_capture_beside_eager(std::initializer_list<const Tensor*> inputs) {
-  if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+  if (!capturing()) return;
   for (const Tensor* t : inputs) {
     if (!t->defined() || !t->requires_grad() || t->grad_fn()) continue;
     const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
@@ -153,7 +155,7 @@ struct LinearBackward : public Node {
     std::lock_guard<std::mutex> lock(mutex_);
     variable_list out(4);
     if (!grads[0].defined()) return out;
-    const Tensor x0 = x.unpack(), w0 = w.unpack(), z0 = act ? z.unpack() : Tensor();
+    const Tensor x0 = x.unpack(), w0 = w.unpack(), z0 = act ? z.unpack(shared_from_this()) : Tensor();
     const bool want_x = task_should_compute_output(0), want_w = task_should_compute_output(1), want_b = task_should_compute_output(2);
     if (task_should_compute_output(3)) out[3] = grads[0];
     {
@@ -219,6 +221,8 @@ Tensor linear(const Tensor& x, const Tensor& w, const MaybeTensor& bias, int64_t
     node = std::shared_ptr<LinearBackward>(new LinearBackward(), torch::autograd::deleteNode);
     node->set_next_edges(torch::autograd::collect_next_edges(x, w, b, r));
   }
+  // (relu's slope can be told from its result, which is kept instead unless a residual was added: one store fewer)
+  const bool from_y = act == MG_ACTIVATION_RELU && !r.defined();
   Tensor y, xm, wm, z;
   {
     at::AutoDispatchBelowADInplaceOrView below;
@@ -228,7 +232,7 @@ Tensor linear(const Tensor& x, const Tensor& w, const MaybeTensor& bias, int64_t
     const int64_t rows = xm.size(0);
     const int dt = dtype_of(type);
     y = make(shape, type, dev);
-    if (node && act) z = make({rows, n}, type, dev);
+    if (node && act && !from_y) z = make({rows, n}, type, dev);
     int64_t need = 0;
     check(L.mg_op_linear_workspace(rows, k, n, dt, &need, nullptr, nullptr));
     const Scratch ws(need, dev);
@@ -238,10 +242,10 @@ Tensor linear(const Tensor& x, const Tensor& w, const MaybeTensor& bias, int64_t
   if (node) {
     node->x = keep(x, xm);
     node->w = keep(w, wm);
-    if (act) node->z = SavedVariable(z, false);
     node->act = act;
     node->x_shape = at::DimVector(x.sizes());
     torch::autograd::set_history(y, node);
+    if (act) node->z = from_y ? SavedVariable(y, true) : SavedVariable(z, false);
   }
   return y;
 }
@@ -268,7 +272,8 @@ void check_logits(const Tensor& l) {
 
 struct PolicyLossBackward : public Node {
   SavedVariable logits, action, mask, save;
-  bool masked = false;
+  Tensor ready;                // the gradient for the factor 1, until a backward pass hands it out
+  bool masked = false, captured = false;
   double ent = 0.0;
   at::DimVector shape;
   std::string name() const override { return "MinigridPolicyLossBackward"; }
@@ -278,6 +283,7 @@ struct PolicyLossBackward : public Node {
     action.reset_data();
     mask.reset_data();
     save.reset_data();
+    ready = Tensor();
   }
   variable_list apply(variable_list&& grads) override {
     std::lock_guard<std::mutex> lock(mutex_);
@@ -288,8 +294,11 @@ struct PolicyLossBackward : public Node {
       at::AutoDispatchBelowADInplaceOrView below;
       const Tensor l = matrix(l0, shape.back());
       const at::Device dev = l.device();
-      out[0] = make(shape, l.scalar_type(), dev);
-      check(L.mg_op_policy_loss_backward(dev.index(), stream_of(dev), dtype_of(l.scalar_type()), l.size(0), l.size(1), ptr(l), row_stride(l), ptr(a0),
+      // (a pass that is captured behind a forward pass that was not would find what it handed out as the caller left it)
+      const bool made = ready.defined() && captured == capturing();
+      out[0] = made ? std::move(ready) : make(shape, l.scalar_type(), dev);
+      ready = Tensor();
+      check((made ? L.mg_op_policy_loss_rescale : L.mg_op_policy_loss_backward)(dev.index(), stream_of(dev), dtype_of(l.scalar_type()), l.size(0), l.size(1), ptr(l), row_stride(l), ptr(a0),
                                          dtype_of(a0.scalar_type()), (const uint8_t*)ptr(m0), ent, ptr(s0), (const float*)ptr(grads[0]), ptr(out[0])));
     }
     return no_second("policy_loss", std::move(out), {&grads[0], &l0});
@@ -312,19 +321,21 @@ std::pair<Tensor, Tensor> policy_loss(const Tensor& logits, const Tensor& action
     node = std::shared_ptr<PolicyLossBackward>(new PolicyLossBackward(), torch::autograd::deleteNode);
     node->set_next_edges(torch::autograd::collect_next_edges(logits));
   }
-  Tensor l, save, loss, stats;
+  Tensor l, save, loss, stats, grad;
   {
     at::AutoDispatchBelowADInplaceOrView below;
     l = matrix(logits, logits.size(-1));
     const int64_t rows = l.size(0), vocab = l.size(1);
     const Tensor out = make({6}, at::kFloat, dev);
     if (node) save = make({rows + 1, 2}, at::kDouble, dev);
+    // (a half-precision loss is scaled before its backward pass: its gradient for the factor 1 would be made in vain)
+    if (node && rows && l.scalar_type() != at::kHalf && L.mg_op_policy_loss_makes_gradient(dtype_of(l.scalar_type()), vocab)) grad = make(logits.sizes(), l.scalar_type(), dev);
     int64_t need = 0;
     check(L.mg_op_policy_loss_workspace(rows, vocab, &need));
     const Scratch ws(need, dev);
-    check(L.mg_op_policy_loss(dev.index(), stream_of(dev), dtype_of(l.scalar_type()), rows, vocab, ptr(l), row_stride(l), ptr(a), dtype_of(a.scalar_type()),
+    check(L.mg_op_policy_loss_with_gradient(dev.index(), stream_of(dev), dtype_of(l.scalar_type()), rows, vocab, ptr(l), row_stride(l), ptr(a), dtype_of(a.scalar_type()),
                               (const float*)ptr(old), (const float*)ptr(adv), (const float*)ptr(ref), (const uint8_t*)ptr(m), lo, hi, kl, ent, (float*)ptr(out), ptr(save),
-                              ws.p(), ws.bytes));
+                              ws.p(), ws.bytes, ptr(grad)));
     loss = out.select(0, 0);
     stats = out.narrow(0, 1, 5);
   }
@@ -334,6 +345,8 @@ std::pair<Tensor, Tensor> policy_loss(const Tensor& logits, const Tensor& action
     node->masked = m.defined();
     if (m.defined()) node->mask = keep(*mask, m);
     node->save = SavedVariable(save, false);
+    node->ready = grad;
+    node->captured = capturing();
     node->ent = ent;
     node->shape = at::DimVector(logits.sizes());
     torch::autograd::set_history(loss, node);

@@ -23,7 +23,7 @@ _ACTIVATIONS = {None: 0, "relu": 1, "tanh": 2, "gelu": 3, "silu": 4}
 
 # every symbol include/minigrid_ops.h declares
 SYMBOLS = ["mg_ops_last_error", "mg_op_linear_workspace", "mg_op_linear", "mg_op_linear_dz_workspace", "mg_op_linear_dz", "mg_op_linear_dx", "mg_op_linear_dw",
-           "mg_op_policy_loss_workspace", "mg_op_policy_loss", "mg_op_policy_loss_backward", "mg_op_sample_workspace", "mg_op_sample", "mg_op_advantages"]
+           "mg_op_policy_loss_workspace", "mg_op_policy_loss", "mg_op_policy_loss_makes_gradient", "mg_op_policy_loss_with_gradient", "mg_op_policy_loss_backward", "mg_op_policy_loss_rescale", "mg_op_sample_workspace", "mg_op_sample", "mg_op_advantages"]
 
 
 class _AdvantagesArgs(C.Structure):
@@ -56,6 +56,9 @@ def _lib():
         L.mg_op_policy_loss_workspace.argtypes = [q, q, pq]
         L.mg_op_policy_loss.argtypes = [i, vp, i, q, q, vp, q, vp, i, vp, vp, vp, vp, d, d, d, d, vp, vp, vp, q]
         L.mg_op_policy_loss_backward.argtypes = [i, vp, i, q, q, vp, q, vp, i, vp, d, vp, vp, vp]
+        L.mg_op_policy_loss_makes_gradient.argtypes = [i, q]
+        L.mg_op_policy_loss_with_gradient.argtypes = L.mg_op_policy_loss.argtypes + [vp]
+        L.mg_op_policy_loss_rescale.argtypes = L.mg_op_policy_loss_backward.argtypes
         L.mg_op_sample_workspace.argtypes = [q, q, pq]
         L.mg_op_sample.argtypes = [i, vp, i, q, q, vp, q, vp, vp, vp, vp, q]
         L.mg_op_advantages.argtypes = [i, vp, C.POINTER(_AdvantagesArgs)]
@@ -91,7 +94,7 @@ def linear(x, weight, bias=None, *, activation: Optional[str] = None, residual=N
     "gelu" (x Phi(x) with the normal distribution function itself) or "silu".  Sums are held in 32 bits and the result is rounded once.
 
     Differentiable in x (unless bytes), weight, bias and residual, once.  For the backward pass of an activation the values in front of it are kept
-    in weight's dtype, and their gradient is rounded to it before the two products that use it (the matrix instructions take such operands);
+    in weight's dtype (relu without a residual: the result itself, which must then not be changed in place), and their gradient is rounded to it before the two products that use it (the matrix instructions take such operands);
     bias's gradient is summed before that rounding.  All sums run in a fixed order."""
     if activation not in _ACTIVATIONS:
         raise ValueError(f"activation must be one of {[a for a in _ACTIVATIONS if a]} or None")
@@ -111,7 +114,8 @@ def policy_loss(logits, action, old_log_prob, advantage, *, mask=None, ref_log_p
 
     Returns (loss, stats): stats are the means of the policy term, the KL term and the entropy, the share of clipped rows, and the number of rows that
     count.  Only the loss is differentiable, in the logits, once.  Rows that do not count are not read, whatever they hold, and get the gradient 0; with
-    no row that counts everything is 0.  Logits of -inf are closed actions.  A counted row whose action is not one of the columns makes the loss NaN."""
+    no row that counts everything is 0.  For more than 64 actions in rows of up to 160 KB of float32 or bfloat16 the gradient is made along with the loss, for the factor 1; a backward
+    pass with another factor (a loss that was scaled) makes it anew.  Logits of -inf are closed actions.  A counted row whose action is not one of the columns makes the loss NaN."""
     lo, hi = clip if isinstance(clip, (tuple, list)) else (clip, clip)
     return (_X or _ext()).policy_loss(logits, action, old_log_prob, advantage, mask, ref_log_prob, float(lo), float(hi), float(kl_coef), float(entropy_coef))
 

@@ -402,6 +402,33 @@ def test_policy_loss_action_outside_is_loud(vocab, action):
     assert bool(loss.isnan()) and bool(d[3].isnan().all()) and not bool(d[:3].isnan().any())
 
 
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("rows,vocab", [(9, 65), (4099, 130), (6, 40961)])
+@pytest.mark.parametrize("masked", [False, True])
+def test_policy_loss_gradient_whatever_the_factor(dt, rows, vocab, masked):
+    """the gradient that is made along with the loss, the one for another factor, and the one of a second pass: factor times the same numbers.  A factor of
+    two changes no rounding (f16: gradients of unmasked sums over a few rows are far above the subnormal numbers only for large factors, which is why they
+    are compared with a tolerance of half its smallest step)"""
+    x, a, old, adv, ref, mask = loss_inputs(rows, vocab, DT[dt], 21)
+    x = x.detach().clone().requires_grad_(True)
+    make = lambda: mg().policy_loss(x, a, old, adv, mask=mask if masked else None, ref_log_prob=ref, kl_coef=0.1, entropy_coef=0.01)[0]
+    one, two = torch.ones((), device="cuda"), torch.full((), 2.0, device="cuda")
+    loss = make()
+    first, = torch.autograd.grad(loss, [x], one, retain_graph=True)
+    kept = first.clone()
+    first.zero_()                                                    # (what was handed out is the caller's)
+    again, = torch.autograd.grad(loss, [x], one, retain_graph=True)
+    twice, = torch.autograd.grad(loss, [x], two)
+    assert torch.equal(again, kept)
+    other, = torch.autograd.grad(make(), [x], two)
+    assert torch.equal(other, twice)
+    assert bool(((twice.double() - 2 * kept.double()).abs() <= (2.0 ** -24 * 1.5 if dt == "f16" else 0)).all())
+    (2 * make()).backward()
+    assert torch.equal(x.grad, twice)
+    if masked:
+        assert not bool(kept[~mask].any())
+
+
 @pytest.mark.parametrize("t", [torch.uint8, torch.int32, torch.int64])
 def test_policy_loss_action_types_and_shapes(t):
     x, a, old, adv, ref, mask = loss_inputs(60, 7, torch.float32, 13, gap=1)
