@@ -809,32 +809,30 @@ template <class T, class S, int ROWS>
 __global__ __launch_bounds__(256) void k_few_rows(int rows, int64_t k, int64_t n, const S* x, int64_t ldx, const T* w, int64_t ldw, Epilogue ep) {
   constexpr int N = Chunk<T>::N;
   const int lane = threadIdx.x & 63;
-  const int64_t j = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (j >= n) return;
-  const T* wj = w + j * ldw;
-  float s[ROWS];
+  for (int64_t j = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); j < n; j += (int64_t)gridDim.x * 4) {
+    const T* wj = w + j * ldw;
+    float s[ROWS];
 #pragma unroll
-  for (int i = 0; i < ROWS; i++) s[i] = 0.0f;
-  for (int64_t c = (int64_t)lane * N; c < k; c += 64 * N) {
-    const auto b = load_chunk<T, T>(wj, c, k, true);
+    for (int i = 0; i < ROWS; i++) s[i] = 0.0f;
+    for (int64_t c = (int64_t)lane * N; c < k; c += 64 * N) {
+      const auto b = load_chunk<T, T>(wj, c, k, true);
 #pragma unroll
-    for (int i = 0; i < ROWS; i++) {
-      if (i < rows) {
-        const auto a = load_chunk<T, S>(x + i * ldx, c, k, true);
+      for (int i = 0; i < ROWS; i++) {
+        if (i < rows) {
+          const auto a = load_chunk<T, S>(x + i * ldx, c, k, true);
 #pragma unroll
-        for (int e = 0; e < N; e++) s[i] = __builtin_fmaf((float)a[e], (float)b[e], s[i]);
+          for (int e = 0; e < N; e++) s[i] = __builtin_fmaf((float)a[e], (float)b[e], s[i]);
+        }
       }
     }
-  }
-  float mine = 0.0f;
+    float mine = 0.0f;
 #pragma unroll
-  for (int i = 0; i < ROWS; i++) {
+    for (int i = 0; i < ROWS; i++) {
 #pragma unroll
-    for (int m = 32; m; m >>= 1) s[i] += __shfl_xor(s[i], m);
-    mine = lane == i ? s[i] : mine;
-  }
-  if (lane < rows) {
-    finish<T>(ep, lane, j, n, mine);
+      for (int m = 32; m; m >>= 1) s[i] += __shfl_xor(s[i], m);
+      mine = lane == i ? s[i] : mine;
+    }
+    if (lane < rows) finish<T>(ep, lane, j, n, mine);
   }
 }
 

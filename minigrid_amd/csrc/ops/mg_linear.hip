@@ -48,7 +48,8 @@ static int product(hipStream_t st, int form, bool bytes, const Operand& A, const
   if (p.tile == TILE_256 && dtype != MG_DT_F32 && !bytes && aligned(A, form == FORM_DW) && aligned(B, form != FORM_FORWARD) && B.extent % 8 == 0 && ep.narrow &&
       row(ep.c, ep.ldc) && row(ep.z, 0) && row(ep.r, ep.ldr) && row(ep.b, 0) && !busy)
     p.tile = TILE_DIRECT;
-  if (ceil_div(A.extent, TILE_I[p.tile]) * ceil_div(B.extent, TILE_J[p.tile]) > 0x7fffffffll) return fail(MG_ERR_INVALID, "the result has too many tiles");
+  // (a launch holds less than 2^32 threads along an axis)
+  if (ceil_div(A.extent, TILE_I[p.tile]) * ceil_div(B.extent, TILE_J[p.tile]) * 512 > 0xffffffffll) return fail(MG_ERR_INVALID, "the result has too many tiles");
   Epilogue first = ep;
   if (p.splits > 1) first.part = (float*)ws;
   return by_type(dtype, [&](auto* t) {
