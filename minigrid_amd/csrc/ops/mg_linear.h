@@ -11,7 +11,7 @@
 //
 // Two kernels.  k_product takes results at least as large as its tile and at least one tile deep, and then needs no bounds check at all: a tile that would
 // stick out is moved back inside (its first rows belong to a neighbour and are not stored), and a last piece of the summed axis is loaded as the last
-// whole one with what was summed already set to zero.  k_product_guarded checks every chunk and takes the rest.
+// whole one with what was summed already set to zero.  k_product_guarded checks the chunks of tiles that are not whole and takes the rest.
 #pragma once
 #include "mg_ops.h"
 
@@ -186,6 +186,14 @@ struct GuardedLoader {
   typename L::V hold[PER];
   __device__ __forceinline__ void load(const Operand& o, int i0, int64_t s0, int64_t send) {
     const S* p = (const S*)o.p;
+    if (i0 + (int64_t)EXT <= o.extent && s0 + L::BK <= send) {      // (uniform: a whole tile, nothing to check)
+#pragma unroll
+      for (int q = 0; q < PER; q++) {
+        const int u = q * THREADS + (int)threadIdx.x, r = u / L::CPR, c = (u % L::CPR) * L::N;
+        hold[q] = load_chunk<T, S>(p + (COLS ? (s0 + r) * o.ld + i0 : (i0 + r) * o.ld + s0), c, (int64_t)1 << 62, true);
+      }
+      return;
+    }
 #pragma unroll
     for (int q = 0; q < PER; q++) {
       const int u = q * THREADS + (int)threadIdx.x, r = u / L::CPR, c = (u % L::CPR) * L::N;
@@ -386,7 +394,8 @@ struct Aligned {                 // rows of elements from (i, j) on
   __device__ __forceinline__ u32x4 get(uint32_t lane, uint32_t at) const { return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, lane, at, 0)); }
   __device__ __forceinline__ void put(bool own, uint32_t lane, uint32_t at, u32x4 d) const { __builtin_amdgcn_raw_buffer_store_b128(d, rsrc, own ? lane : OUTSIDE, at, 0); }
 };
-// Inside: a tile that owns all of its rows and columns, at any alignment
+// Inside: a whole tile at any alignment.  (Eight columns of which only the last are a tile's own are stored by its neighbour too: the same sums in the
+// same order, so the same bits.)
 struct Inside {
   char* base;
   uint32_t row;
@@ -396,7 +405,9 @@ struct Inside {
     __builtin_memcpy(&d, base + at + lane, 16);
     return d;
   }
-  __device__ __forceinline__ void put(bool, uint32_t lane, uint32_t at, u32x4 d) const { __builtin_memcpy(base + at + lane, &d, 16); }
+  __device__ __forceinline__ void put(bool own, uint32_t lane, uint32_t at, u32x4 d) const {
+    if (own) __builtin_memcpy(base + at + lane, &d, 16);
+  }
 };
 
 // The sums pass through LDS as in store_tile, up to 64 rows at a time, and a lane ends with the same eight columns of every (64 / LPR)-th row.  (A row's
@@ -408,7 +419,7 @@ __device__ __forceinline__ void store_wave(const Epilogue& ep, f32x16 (&acc)[MI]
   typedef T V8 __attribute__((ext_vector_type(8)));
   constexpr int COLS = MJ * 32, LPR = COLS / 8, RPP = 64 / LPR, H = MI > 2 ? MI / 2 : 1, MH = MI / H, P = MH * 32 / RPP, SZ = sizeof(T), SWAP = MJ > 1 ? 32 : 0;
   const int l = threadIdx.x & 63, r0 = l / LPR, col = (l % LPR) * 8;
-  const bool mine = col >= jown;
+  const bool mine = col + 8 > jown;
   auto put_stage = [&](int h) __attribute__((always_inline)) {
 #pragma unroll
     for (int a = 0; a < MH; a++)
@@ -610,13 +621,7 @@ __global__ __launch_bounds__(WI * WJ * 64) void k_product(Operand A, Operand B, 
   static_assert(WI * WJ * 32 * (MJ * 32 + 8) * 4 <= (int)sizeof lds, "staging fits");
   constexpr int STAGED = (MI > 2 ? 64 : MI * 32) * MJ * 32;
   static_assert(WI * WJ * STAGED * 4 <= (int)sizeof lds, "staging fits");
-  // (the kernel has the registers for one epilogue without branches: inside tiles, all but the last row and column of tiles; 32-bit offsets within a tile)
-  if (i0 == at.i * BI && j0 == at.j * BJ && ep.narrow) {
-    store_wave_any<T, BCOLS, Inside, MI, MJ>(ep, acc, (float*)lds + wave * STAGED, i0 + wi, 0, j0 + wj, 0, A.extent, B.extent);
-    return;
-  }
-  float* stage = (float*)lds + wave * 32 * (MJ * 32 + 8);
-  store_tile_any<T, BCOLS, MI, MJ>(ep, acc, stage, i0 + wi, at.i * (int64_t)BI, A.extent, j0 + wj, at.j * (int64_t)BJ, B.extent);
+  store_wave_any<T, BCOLS, Inside, MI, MJ>(ep, acc, (float*)lds + wave * STAGED, i0 + wi, at.i * BI - i0 - wi, j0 + wj, at.j * BJ - j0 - wj, A.extent, B.extent);
 }
 
 // An operand's tile from memory straight into LDS, 16 bytes a lane: no registers in between, and nothing waits for it but the wait that is written down.
@@ -770,7 +775,9 @@ __global__ __launch_bounds__(WI * WJ * 64) void k_product_guarded(Operand A, Ope
   constexpr int BK = LA::BK, BUF = LA::BYTES + LB::BYTES;
   __shared__ __attribute__((aligned(16))) char lds[2 * BUF];
   const TileAt at = tile_at((A.extent + BI - 1) / BI, (B.extent + BJ - 1) / BJ);
-  const int i0 = at.i * BI, j0 = at.j * BJ;
+  // (whole tiles where there are some: the last ones are moved back inside)
+  const bool whole = A.extent >= BI && B.extent >= BJ && ep.narrow;
+  const int i0 = whole ? min(at.i * BI, A.extent - BI) : at.i * BI, j0 = whole ? min(at.j * BJ, B.extent - BJ) : at.j * BJ;
   const int64_t s_begin = (int64_t)blockIdx.y * tiles_per_split * BK, s_end = min(depth, s_begin + (int64_t)tiles_per_split * BK);
   const int wave = threadIdx.x >> 6, wi = (wave / WJ) * (BI / WI), wj = (wave % WJ) * (BJ / WJ);
   f32x16 acc[MI][MJ];
@@ -798,7 +805,12 @@ __global__ __launch_bounds__(WI * WJ * 64) void k_product_guarded(Operand A, Ope
     cur ^= 1;
   }
   __syncthreads();
-  static_assert(WI * WJ * 32 * (MJ * 32 + 8) * 4 <= (int)sizeof lds, "staging fits");
+  constexpr int STAGED = (MI > 2 ? 64 : MI * 32) * MJ * 32;
+  static_assert(WI * WJ * STAGED * 4 <= (int)sizeof lds && WI * WJ * 32 * (MJ * 32 + 8) * 4 <= (int)sizeof lds, "staging fits");
+  if (whole) {
+    store_wave_any<T, BCOLS, Inside, MI, MJ>(ep, acc, (float*)lds + wave * STAGED, i0 + wi, at.i * BI - i0 - wi, j0 + wj, at.j * BJ - j0 - wj, A.extent, B.extent);
+    return;
+  }
   float* stage = (float*)lds + wave * 32 * (MJ * 32 + 8);
   store_tile_any<T, BCOLS, MI, MJ>(ep, acc, stage, i0 + wi, 0, A.extent, j0 + wj, 0, B.extent);
 }

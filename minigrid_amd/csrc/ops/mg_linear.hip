@@ -36,8 +36,8 @@ static int product(hipStream_t st, int form, bool bytes, const Operand& A, const
   ep.narrow = std::max({ep.ldc, ep.r ? ep.ldr : 0, (int64_t)B.extent}) < (1 << 21);
   Plan p = plan_product(A.extent, B.extent, depth, dtype);
   if (p.part_bytes > ws_bytes || (p.part_bytes && (!ws || ((uintptr_t)ws & 255)))) return fail(MG_ERR_INVALID, "workspace: %lld bytes, 256-byte aligned, are needed", (long long)p.part_bytes);
-  // (rows so far apart that a tile of them spans 2 GiB: the kernel with 64-bit offsets, same splits)
-  if (p.tile >= TILE_64 && std::max(A.ld, B.ld) * TILE_I[p.tile] * 4 >= 0x7fffffffll) p.tile = TILE_GUARDED_128_128;
+  // (rows so far apart that a tile of them, or of the result, spans 2 GiB: the kernel with 64-bit offsets, same splits)
+  if (p.tile >= TILE_64 && (!ep.narrow || std::max(A.ld, B.ld) * TILE_I[p.tile] * 4 >= 0x7fffffffll)) p.tile = TILE_GUARDED_128_128;
   // Four waves of 128 x 128 or eight of 128 x 64?  The four multiply faster (65 536 x 1024 x 512: 69 us against 78; 32 768 x 2048 x 4096: 448 against 521),
   // the eight get a tile's z and residual through faster, which decides up to 512 summed elements (65 536 x 256 x 512 with both: 61 us against 54,
   // 65 536 x 512 x 512 from cold memory: 99 against 87; 65 536 x 768 x 512: 95 against 102).
