@@ -755,6 +755,60 @@ def test_saved_tensor_hooks_and_checkpointing():
     assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(y, [x, w, b, r], dy), want))
 
 
+def test_relu_keeps_its_result():
+    """without a residual the backward pass reads relu's result: through hooks and checkpoints the same gradients, and a change of it in place is noticed"""
+    x, w, b, _, dy = linear_inputs(70, 24, 40, torch.bfloat16, False, True, False, True, 6)
+    for t in (x, w, b):
+        t.requires_grad_(True)
+    f = lambda *t: mg().linear(*t, activation="relu")
+    want = torch.autograd.grad(mg().linear(x, w, b, activation="relu", residual=torch.zeros_like(dy)), [x, w, b], dy)
+    assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(f(x, w, b), [x, w, b], dy), want))
+    with torch.autograd.graph.save_on_cpu():
+        y = f(x, w, b)
+    assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(y, [x, w, b], dy), want))
+    from torch.utils.checkpoint import checkpoint
+    y = checkpoint(f, x, w, b, use_reentrant=False)
+    assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(y, [x, w, b], dy), want))
+    y = f(x.view(7, 10, 24), w, b)
+    assert torch.equal(torch.autograd.grad(y, [x], dy.view(7, 10, 40))[0], want[0])
+    y = f(x, w, b)
+    with torch.no_grad():
+        y.add_(1)
+    with pytest.raises(RuntimeError, match="inplace"):
+        torch.autograd.grad(y, [x], dy)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+def test_long_rows_captured_and_replayed(dt):
+    """the gradient that comes with the loss is made anew by every replay, whatever the caller did to the one before"""
+    x, a, old, adv, ref, mask = loss_inputs(37, 700, DT[dt], 4)
+    x = x.detach().clone().requires_grad_(True)
+    scale = torch.ones((), device="cuda")
+
+    def step():
+        loss, stats = mg().policy_loss(x, a, old, adv, mask=mask, ref_log_prob=ref, kl_coef=0.1, entropy_coef=0.01)
+        d, = torch.autograd.grad(loss, [x], scale)
+        return loss.detach(), stats, d
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step()
+    for i in range(5):
+        scale.fill_(1.0 if i % 2 else 0.5 + i)
+        adv.copy_(torch.randn(adv.shape, generator=gen(50 + i), device="cuda"))
+        mask.copy_(torch.rand(mask.shape, generator=gen(60 + i), device="cuda") < 0.7)
+        want = step()
+        out[2].zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(want, out)), i
+
+
 # ---- refusals ---------------------------------------------------------------------------------------------------------------------------
 
 def test_refusals():
