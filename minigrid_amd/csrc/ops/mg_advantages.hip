@@ -168,8 +168,9 @@ int mg_op_advantages(int device, void* stream, const mg_advantages_args* args) {
                     g.s_term[0] % 2 == 0 && g.s_term[1] % 2 == 0;
   const bool record = pair && g.reward_dtype == MG_DT_F64 && (const uint8_t*)g.reward + 8 == g.terminated && !((uintptr_t)g.reward & 15) && g.s_reward[0] % 2 == 0 &&
                       g.s_reward[1] % 2 == 0 && g.s_term[0] == 8 * g.s_reward[0] && g.s_term[1] == 8 * g.s_reward[1];
-  // As many environments per workgroup as leave every CU one; a short rollout has nothing to spread over the lanes.
-  const int el = g.envs >= 64 * 256 || g.steps <= SEG ? 64 : g.envs >= 16 * 128 || g.steps <= 4 * SEG ? 16 : 4;
+  // As many environments per workgroup as leave every CU two, or half of them one (128 x 20 000: 20 us with 16, 25 with 64; 53 x 58 162: 37 and 30;
+  // 300 x 1 000: 13 with 4, 11 with 16, 22 with 64; 1 788 x 2: 13, 40 and 130); a short rollout has nothing to spread over the lanes.
+  const int el = g.envs >= 64 * 512 || g.steps <= SEG ? 64 : g.envs >= 16 * 128 || g.steps <= 4 * SEG ? 16 : 4;
   const int64_t stretches = (g.steps + SEG - 1) / SEG;
   const int waves = (int)std::min<int64_t>(WAVES, (stretches * el + 63) / 64);
   const unsigned grid = (unsigned)((g.envs + el - 1) / el);

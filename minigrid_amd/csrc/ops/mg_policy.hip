@@ -550,12 +550,16 @@ __global__ void k_sample_small(const T* logits, int64_t ld, int64_t rows_all, in
 
 // Long rows: a row is cut into 64 pieces, a wave per piece finds its maximum and its sum against it; from the 64 pairs one wave finds the piece in which the
 // running sum passes the border, and walks that piece alone.  Few rows: the pieces of a row are dealt to up to sixteen workgroups, and a second kernel
-// walks; many rows: one workgroup of four waves does both.  Bound by memory for many rows, by two short launches for few.
+// walks; more rows: one workgroup of four waves does both; many: a wave does.  Bound by the 64-bit exponentials for many rows, by two short launches for few.
 constexpr int PIECES = 64, E = 4;        // E: elements of a lane at a time
 struct Piece { float m; int32_t at; double s; };          // the largest logit, its first index, sum e^{l - m}
 static_assert(sizeof(Piece) == 16, "the workspace is counted in these");
 
-__device__ __forceinline__ int64_t piece_length(int64_t vocab) { return ((vocab + PIECES - 1) / PIECES + E - 1) / E * E; }
+// (a piece is at least what a wave reads at once: 256 elements; the pieces behind the row's end are empty)
+__host__ __device__ __forceinline__ int64_t piece_length(int64_t vocab) {
+  const int64_t n = ((vocab + PIECES - 1) / PIECES + E - 1) / E * E;
+  return n < 64 * E ? 64 * E : n;
+}
 
 template <class T>
 __device__ __forceinline__ void load_some(const T* row, int64_t c, int64_t to, float (&x)[E]) {
@@ -667,17 +671,17 @@ __device__ __forceinline__ void choose(const T* row, int64_t vocab, Piece mine, 
   }
 }
 
-// grid (rows, groups): group g looks at its 64 / groups pieces of a row; a single group chooses at once
+// grid (rows, groups): every wave of a row's groups looks at every (4 groups)-th piece; a single group chooses at once
 template <class T>
 __global__ __launch_bounds__(256) void k_sample_rows(const T* logits, int64_t ld, int64_t rows, int64_t vocab, const float* u, Piece* pieces, void* action, float* lp) {
   __shared__ Piece all[PIECES];
-  const int w = threadIdx.x >> 6, n = PIECES / gridDim.y, first = blockIdx.y * n;
+  const int w = threadIdx.x >> 6;
   const int64_t len = piece_length(vocab);
   for (int64_t i = blockIdx.x; i < rows; i += gridDim.x) {
     const T* row = logits + i * ld;
-    for (int p = first + w; p < first + n; p += 4) {
+    for (int p = blockIdx.y * 4 + w; p < PIECES; p += 4 * gridDim.y) {
       const int64_t from = min(vocab, p * len), to = min(vocab, from + len);
-      const Piece q = look_at(row, from, to);
+      const Piece q = from < to ? look_at(row, from, to) : Piece{NEG_INF, 0, 0.0};
       if ((threadIdx.x & 63) == 0) {
         if (pieces) pieces[i * PIECES + p] = q;
         else all[p] = q;
@@ -690,6 +694,21 @@ __global__ __launch_bounds__(256) void k_sample_rows(const T* logits, int64_t ld
   }
 }
 
+// Many rows, or short ones: a wave per row, so that none waits for another
+template <class T>
+__global__ __launch_bounds__(256) void k_sample_waves(const T* logits, int64_t ld, int64_t rows, int64_t vocab, const float* u, void* action, float* lp) {
+  const int64_t len = piece_length(vocab);
+  for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); i < rows; i += (int64_t)gridDim.x * 4) {
+    const T* row = logits + i * ld;
+    Piece mine = {NEG_INF, 0, 0.0};
+    for (int p = 0; p * len < vocab; p++) {
+      const Piece q = look_at(row, p * len, min(vocab, (p + 1) * len));
+      if ((int)(threadIdx.x & 63) == p) mine = q;
+    }
+    choose(row, vocab, mine, i, u, action, lp);
+  }
+}
+
 template <class T>
 __global__ __launch_bounds__(64) void k_sample_choose(const T* logits, int64_t ld, int64_t vocab, const float* u, const Piece* pieces, void* action, float* lp) {
   const int64_t i = blockIdx.x;
@@ -697,11 +716,16 @@ __global__ __launch_bounds__(64) void k_sample_choose(const T* logits, int64_t l
 }
 
 // workgroups per row: four of them a CU, each of its four waves with at least one piece (64 x 40 961 f32: 10.5 us with two of them a CU)
-static int sample_groups(int64_t rows) {
+static int sample_groups(int64_t rows, int64_t vocab) {
+  const int64_t pieces = (vocab + piece_length(vocab) - 1) / piece_length(vocab);
   int g = 1;
-  while (g < PIECES / 4 && rows * g < 1024) g *= 2;
+  while (g * 4 < pieces && rows * g < 1024) g *= 2;
   return g;
 }
+
+// A wave per row, or a workgroup (or several)?  4 096 x 1 000: 16 us against 33, 262 144 x 100: 361 against 1 682, 16 384 x 4 096: 139 against 200; for fewer
+// rows only where they are short: 512 x 197: 6.7 against 8.4, 1 024 x 5 000: 29 against 20, 2 048 x 32 000: 165 against 126.
+static bool wave_per_row(int64_t rows, int64_t vocab) { return rows >= 4096 || (rows >= 512 && vocab <= 1024); }
 
 static int check_logits(int dtype, int64_t rows, int64_t vocab, int64_t ld) {
   if (dtype != MG_DT_F32 && dtype != MG_DT_BF16 && dtype != MG_DT_F16) return fail(MG_ERR_INVALID, "logits must be f32, bf16 or f16");
@@ -833,7 +857,7 @@ int mg_op_sample_workspace(int64_t rows, int64_t vocab, int64_t* bytes) {
   const int rc = check_logits(MG_DT_F32, rows, vocab, vocab);
   if (rc != MG_OK) return rc;
   if (!bytes) return fail(MG_ERR_INVALID, "bytes must not be NULL");
-  *bytes = vocab > SMALL_VOCAB && sample_groups(rows) > 1 ? rows * PIECES * (int64_t)sizeof(Piece) : 0;
+  *bytes = vocab > SMALL_VOCAB && !wave_per_row(rows, vocab) && sample_groups(rows, vocab) > 1 ? rows * PIECES * (int64_t)sizeof(Piece) : 0;
   return MG_OK;
 }
 
@@ -854,8 +878,10 @@ int mg_op_sample(int device, void* stream, int dtype, int64_t rows, int64_t voca
     if (vocab <= SMALL_VOCAB) {
       const int R = small_rows(vocab);
       k_sample_small<T><<<(unsigned)((rows + R - 1) / R), R, (size_t)R * (vocab | 1) * 4, st>>>(x, ld, rows, (int)vocab, u, action, lp);
+    } else if (wave_per_row(rows, vocab)) {
+      k_sample_waves<T><<<(unsigned)std::min<int64_t>((rows + 3) / 4, 1 << 22), 256, 0, st>>>(x, ld, rows, vocab, u, action, lp);
     } else {
-      const int groups = sample_groups(rows);
+      const int groups = sample_groups(rows, vocab);
       Piece* pieces = groups > 1 ? (Piece*)ws : nullptr;
       k_sample_rows<T><<<dim3((unsigned)std::min<int64_t>(rows, 1 << 22), groups), 256, 0, st>>>(x, ld, rows, vocab, u, pieces, action, lp);
       if (pieces) k_sample_choose<T><<<(unsigned)rows, 64, 0, st>>>(x, ld, vocab, u, pieces, action, lp);

@@ -507,6 +507,14 @@ def test_sample_actions(dt, rows, vocab, greedy):
     within(lp, wlp, 2 * U * wlp.abs() + 1e-9, "log_prob")
 
 
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("rows,vocab", [(512, 197), (513, 1024), (600, 1025), (4097, 66), (4100, 1500), (2, 255), (70, 256), (70, 513), (1100, 2600)])
+@pytest.mark.parametrize("greedy", [False, True])
+def test_sample_actions_ways(dt, rows, vocab, greedy):
+    """a wave per row, a workgroup per row, several workgroups per row; pieces that are empty, whole, or hold one element"""
+    test_sample_actions(dt, rows, vocab, greedy)
+
+
 @pytest.mark.parametrize("vocab", [7, 300, 20000])
 def test_sample_actions_edges(vocab):
     g = gen(vocab)
