@@ -9,14 +9,15 @@ static bool fits(int tile, int64_t ri, int64_t rj, int64_t depth, int bk) { retu
 
 // The largest tile with which the CUs are busy, the summed axis split where the tiles of the result alone do not do that (in runs of at least four tiles).
 // A CU holds one workgroup of the 256-tile, two of 128, four of 64.  Where the 256-tiles would have to be split and the 128-tiles fill the CUs by themselves, those:
-// 3 297 x 1 483 x 2 096 66 us against 58, 6 000 x 3 003 x 1 001 86 against 72; at 256 tiles of 128 the split 256-tiles are ahead (1 024 x 4 096 x 4 096 58 against 66).
+// 3 297 x 1 483 x 2 096 66 us against 58, 6 000 x 3 003 x 1 001 86 against 72; at 256 tiles of 128 the split 256-tiles are ahead (1 024 x 4 096 x 4 096 58 against 66),
+// and along a long axis (4 096 x 32 768 x 2 048 467 against 770).
 static Plan plan_product(int64_t ri, int64_t rj, int64_t depth, int dtype) {
   Plan p;
   const int bk = 128 / dtype_bytes(dtype);
   const int64_t deep = ceil_div(depth, bk);
   auto tiles = [&](int t) { return ceil_div(ri, TILE_I[t]) * ceil_div(rj, TILE_J[t]); };
   int64_t slots;
-  if (fits(TILE_256, ri, rj, depth, bk) && tiles(TILE_256) * deep >= 256 * 8 && (tiles(TILE_256) >= 200 || tiles(TILE_128) < 300)) { p.tile = TILE_256; slots = 256; }
+  if (fits(TILE_256, ri, rj, depth, bk) && tiles(TILE_256) * deep >= 256 * 8 && (tiles(TILE_256) >= 200 || tiles(TILE_128) < 300 || deep > 64)) { p.tile = TILE_256; slots = 256; }
   else if (fits(TILE_128, ri, rj, depth, bk) && tiles(TILE_128) * deep >= 256 * 4) { p.tile = TILE_128; slots = 512; }
   else if (fits(TILE_64, ri, rj, depth, bk)) { p.tile = TILE_64; slots = 1024; }
   else { p.tile = ri <= 32 ? TILE_GUARDED_32_128 : rj <= 32 ? TILE_GUARDED_128_32 : TILE_GUARDED_128_128; slots = 512; }
