@@ -7,11 +7,13 @@
 //
 // An operand that is contiguous along s ("rows") lies in LDS as 128-byte rows of one tile row each; one that is contiguous along i / j ("cols") lies
 // there as one row per s and is turned by the transposing LDS read (16-bit types) or read element by element (f32).  Both are swizzled so that the
-// fragment reads of a wave spread over all banks.  Global loads go through registers: rows may start at any address, and bytes are widened on the way.
+// fragment reads of a wave spread over all banks.
 //
-// Two kernels.  k_product takes results at least as large as its tile and at least one tile deep, and then needs no bounds check at all: a tile that would
+// Three kernels.  k_product takes results at least as large as its tile and at least one tile deep, and then needs no bounds check at all: a tile that would
 // stick out is moved back inside (its first rows belong to a neighbour and are not stored), and a last piece of the summed axis is loaded as the last
-// whole one with what was summed already set to zero.  k_product_guarded checks the chunks of tiles that are not whole and takes the rest.
+// whole one with what was summed already set to zero.  Its global loads go through registers: rows may start at any address, and bytes are widened on the
+// way.  k_product_direct is the 256-tile of it whose rows are 16-byte aligned: memory to LDS without registers in between.  k_product_guarded checks the
+// chunks of tiles that are not whole and takes the rest.
 #pragma once
 #include "mg_ops.h"
 

@@ -190,6 +190,19 @@ def test_linear_strides_and_offsets(dt):
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
 
 
+def test_linear_rows_far_apart():
+    """rows of the residual 2^21 elements apart, of x 2^23: more than 32-bit offsets within a tile reach; the same numbers as from packed copies"""
+    rows, k, n = 300, 136, 264
+    x, w, b, r, dy = linear_inputs(rows, k, n, torch.bfloat16, False, True, True, False, 13)
+    for shift in (21, 23):
+        far = torch.empty((rows, 1 << shift), dtype=torch.bfloat16, device="cuda")
+        far[:, :n] = r
+        far[:, n:n + k] = x
+        want = run_linear(x, w, b, r, dy, "gelu")
+        for got in (run_linear(x, w, b, far[:, :n], dy, "gelu"), run_linear(far[:, n:n + k], w, b, r, dy, "gelu")):
+            assert all(torch.equal(p, q) for p, q in zip(want, got)), shift
+
+
 def test_linear_against_differences():
     g = gen(11)
     f = lambda *s: torch.randn(s, generator=g, device="cuda")

@@ -86,9 +86,17 @@ def test_c_entries_refuse_before_the_device_is_touched():
     _rc(loss(ws=None), "workspace")
     _rc(loss(wsb=8), "workspace")
     _rc(L.mg_op_policy_loss_backward(0, None, 0, 4, 7, p, 7, p, 6, None, 0.0, None, p, p), "NULL")
+    # the gradient comes with the loss for rows of more than 64 columns and at most 160 KB
+    with_gradient = lambda dt, vocab: L.mg_op_policy_loss_with_gradient(0, None, dt, 4, vocab, p, vocab, p, 6, p, p, None, None, 0.2, 0.2, 0.0, 0.0, p, None, p, 1 << 20, p)
+    for dt, vocab, makes in ((0, 7, 0), (0, 64, 0), (0, 65, 1), (0, 40960, 1), (0, 40961, 0), (1, 81920, 1), (1, 81921, 0)):
+        assert L.mg_op_policy_loss_makes_gradient(dt, vocab) == makes, (dt, vocab)
+        if not makes:
+            _rc(with_gradient(dt, vocab), "no gradient comes with the loss")
+            _rc(L.mg_op_policy_loss_rescale(0, None, dt, 4, vocab, p, vocab, p, 6, None, 0.0, p, p, p), "no gradient comes with the loss")
+    _rc(L.mg_op_policy_loss_rescale(0, None, 0, 4, 65, p, 65, p, 6, None, 0.0, None, p, p), "NULL")
     _rc(L.mg_op_sample(0, None, 0, 4, 7, p, 6, None, p, p, None, 0), "row stride")
     _rc(L.mg_op_sample(0, None, 0, 4, 7, p, 7, None, None, p, None, 0), "NULL")
-    _rc(L.mg_op_sample(0, None, 0, 4, 300, p, 300, None, p, p, None, 0), "workspace")
+    _rc(L.mg_op_sample(0, None, 0, 4, 3000, p, 3000, None, p, p, None, 0), "workspace")
     assert L.mg_op_sample(0, None, 0, 0, 7, None, 7, None, None, None, None, 0) == B.MG_OK
     _rc(L.mg_op_advantages(0, None, None), "args")
     a = ops._AdvantagesArgs(steps=2, envs=3)
