@@ -441,11 +441,12 @@ __device__ __forceinline__ void store_wave(const Epilogue& ep, f32x16 (&acc)[MI]
 #pragma unroll 4
       for (int p = 0; p < P; p++) {
         const int row = p * RPP + r0;
-        const u32x4 lo = *(const u32x4*)staged(row), hi = *(const u32x4*)(staged(row) + 4);
+        u32x4 sums[2];
+        __builtin_memcpy(sums, __builtin_assume_aligned(staged(row), 16), sizeof sums);
         const bool own = mine && h * MH * 32 + row >= iown;
         const uint32_t at = (h * P + p) * RPP * part.row;
-        part.put(own, off, at, lo);
-        part.put(own, off + 16, at, hi);
+        part.put(own, off, at, sums[0]);
+        part.put(own, off + 16, at, sums[1]);
       }
       __builtin_amdgcn_wave_barrier();
     }
@@ -480,8 +481,7 @@ __device__ __forceinline__ void store_wave(const Epilogue& ep, f32x16 (&acc)[MI]
   auto finish_row = [&](int h, int p, const u32x4 (&residual)[W]) __attribute__((always_inline)) {
     const int row = p * RPP + r0;
     float v[8];
-    *(u32x4*)v = *(const u32x4*)staged(row);
-    *(u32x4*)(v + 4) = *(const u32x4*)(staged(row) + 4);
+    __builtin_memcpy(v, __builtin_assume_aligned(staged(row), 16), sizeof v);
     const bool own = mine && h * MH * 32 + row >= iown;
     const uint32_t step = (h * P + p) * RPP;
     V8 t, add;
