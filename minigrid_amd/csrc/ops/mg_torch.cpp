@@ -8,7 +8,7 @@
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
 
-#include <c10/hip/HIPGraphsC10Utils.h>
+#include <c10/hip/HIPException.h>
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>
 
@@ -122,12 +122,18 @@ variable_list no_second(const char* name, variable_list&& grads, std::initialize
   return std::move(grads);
 }
 
-bool capturing() { return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None; }
+// the capture that the device's current stream takes part in: a number that no other capture has, or 0
+uint64_t capture_on(at::Device dev) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  C10_HIP_CHECK(hipStreamGetCaptureInfo(c10::hip::getCurrentHIPStream(dev.index()).stream(), &status, &id));
+  return status == hipStreamCaptureStatusNone ? 0 : id;
+}
 
 // A captured step must not meet an eager graph of the same leaves that is still alive: the leaves' gradient nodes belong to the stream that graph was recorded
 // on, the backward pass would wait on that stream from inside the capture, and torch ends the process there.  Said here, where it can still be said.
-void refuse_capture_beside_eager(std::initializer_list<const Tensor*> inputs) {
-  if (!capturing()) return;
+void refuse_capture_beside_eager(at::Device dev, std::initializer_list<const Tensor*> inputs) {
+  if (!capture_on(dev)) return;
   for (const Tensor* t : inputs) {
     if (!t->defined() || !t->requires_grad() || t->grad_fn()) continue;
     const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
@@ -217,7 +223,7 @@ Tensor linear(const Tensor& x, const Tensor& w, const MaybeTensor& bias, int64_t
   }
   std::shared_ptr<LinearBackward> node;
   if (at::GradMode::is_enabled() && torch::autograd::compute_requires_grad(x, w, b, r)) {
-    refuse_capture_beside_eager({&x, &w, &b, &r});
+    refuse_capture_beside_eager(dev, {&x, &w, &b, &r});
     node = std::shared_ptr<LinearBackward>(new LinearBackward(), torch::autograd::deleteNode);
     node->set_next_edges(torch::autograd::collect_next_edges(x, w, b, r));
   }
@@ -273,7 +279,8 @@ void check_logits(const Tensor& l) {
 struct PolicyLossBackward : public Node {
   SavedVariable logits, action, mask, save;
   Tensor ready;                // the gradient for the factor 1, until a backward pass hands it out
-  bool masked = false, captured = false;
+  bool masked = false;
+  uint64_t capture = 0;        // that the forward pass belongs to
   double ent = 0.0;
   at::DimVector shape;
   std::string name() const override { return "MinigridPolicyLossBackward"; }
@@ -294,8 +301,9 @@ struct PolicyLossBackward : public Node {
       at::AutoDispatchBelowADInplaceOrView below;
       const Tensor l = matrix(l0, shape.back());
       const at::Device dev = l.device();
-      // (a pass that is captured behind a forward pass that was not would find what it handed out as the caller left it)
-      const bool made = ready.defined() && captured == capturing();
+      // (a pass that is captured behind a forward pass outside of its own capture may be replayed several times behind one forward pass, and would then find
+      // what it handed out before, as the caller left it)
+      const bool made = ready.defined() && capture == capture_on(dev);
       out[0] = made ? std::move(ready) : make(shape, l.scalar_type(), dev);
       ready = Tensor();
       check((made ? L.mg_op_policy_loss_rescale : L.mg_op_policy_loss_backward)(dev.index(), stream_of(dev), dtype_of(l.scalar_type()), l.size(0), l.size(1), ptr(l), row_stride(l), ptr(a0),
@@ -317,7 +325,7 @@ std::pair<Tensor, Tensor> policy_loss(const Tensor& logits, const Tensor& action
                m = mask ? per_row("mask", *mask, lead, dev, {at::kBool, at::kByte}) : Tensor();
   std::shared_ptr<PolicyLossBackward> node;
   if (at::GradMode::is_enabled() && logits.requires_grad()) {
-    refuse_capture_beside_eager({&logits});
+    refuse_capture_beside_eager(dev, {&logits});
     node = std::shared_ptr<PolicyLossBackward>(new PolicyLossBackward(), torch::autograd::deleteNode);
     node->set_next_edges(torch::autograd::collect_next_edges(logits));
   }
@@ -346,7 +354,7 @@ std::pair<Tensor, Tensor> policy_loss(const Tensor& logits, const Tensor& action
     if (m.defined()) node->mask = keep(*mask, m);
     node->save = SavedVariable(save, false);
     node->ready = grad;
-    node->captured = capturing();
+    node->capture = capture_on(dev);
     node->ent = ent;
     node->shape = at::DimVector(logits.sizes());
     torch::autograd::set_history(loss, node);

@@ -1,0 +1,42 @@
+"""Calls of the learning operators that their own sizes, masks and types do not reach: two captures, lazily negated tensors, saved-tensor hooks, ratios next to the
+clipping border, rollouts one after the other."""
+import math
+import pickle
+
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+from test_gpu_ops import DT, U, advantages64, check_loss, gen, linear_inputs, loss_inputs, mg, within
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+def test_policy_loss_backward_in_a_graph_of_its_own(dt):
+    """the loss in one graph, its backward pass in another that is replayed several times behind one replay of the first: every replay gives the gradient of the
+    factor that it finds, whatever the one before left and the caller did to it"""
+    x, a, old, adv, ref, mask = loss_inputs(37, 700, DT[dt], 4)
+    x = x.detach().clone().requires_grad_(True)
+    scale = torch.ones((), device="cuda")
+    make = lambda: mg().policy_loss(x, a, old, adv, mask=mask, ref_log_prob=ref, kl_coef=0.1, entropy_coef=0.01)[0]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        torch.autograd.grad(make(), [x], scale)
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    forward, backward = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(forward):
+        loss = make()
+    with torch.cuda.graph(backward, pool=forward.pool()):
+        d, = torch.autograd.grad(loss, [x], scale, retain_graph=True)
+    want = {f: torch.autograd.grad(make(), [x], torch.full((), f, device="cuda"))[0] for f in (1.0, 2.0)}
+    for i in range(2):
+        forward.replay()
+        for f, spoil in ((1.0, False), (2.0, False), (1.0, False), (1.0, True), (2.0, True), (1.0, False)):
+            scale.fill_(f)
+            if spoil:
+                d.fill_(7.0)
+            backward.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(d, want[f]), (i, f, spoil)
