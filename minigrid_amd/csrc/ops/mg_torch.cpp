@@ -144,6 +144,12 @@ void refuse_capture_beside_eager(at::Device dev, std::initializer_list<const Ten
   }
 }
 
+// There is no forward-mode derivative: a result without a tangent would be taken for a constant.
+void refuse_tangents(const char* name, std::initializer_list<const Tensor*> inputs) {
+  for (const Tensor* t : inputs)
+    if (t->defined() && torch::autograd::isFwGradDefined(*t)) refuse(name, " has no forward-mode derivative: an argument carries a tangent");
+}
+
 // ---- linear ---------------------------------------------------------------------------------------------------------------------------
 
 struct LinearBackward : public Node {
@@ -161,6 +167,7 @@ struct LinearBackward : public Node {
     std::lock_guard<std::mutex> lock(mutex_);
     variable_list out(4);
     if (!grads[0].defined()) return out;
+    refuse_tangents("the gradient of linear", {&grads[0]});
     const Tensor x0 = x.unpack(), w0 = w.unpack(), z0 = act ? z.unpack(shared_from_this()) : Tensor();
     const bool want_x = task_should_compute_output(0), want_w = task_should_compute_output(1), want_b = task_should_compute_output(2);
     if (task_should_compute_output(3)) out[3] = grads[0];
@@ -203,6 +210,8 @@ struct LinearBackward : public Node {
 };
 
 Tensor linear(const Tensor& x, const Tensor& w, const MaybeTensor& bias, int64_t act, const MaybeTensor& residual) {
+  const Tensor b = bias.value_or(Tensor()), r = residual.value_or(Tensor());
+  refuse_tangents("linear", {&x, &w, &b, &r});
   on_gpu("weight", w);
   const at::Device dev = w.device();
   on_gpu("x", x, dev);
@@ -211,7 +220,6 @@ Tensor linear(const Tensor& x, const Tensor& w, const MaybeTensor& bias, int64_t
   const int64_t n = w.size(0), k = w.size(1);
   if (x.scalar_type() != type && x.scalar_type() != at::kByte) refuse("x must be ", type, " (weight's dtype) or uint8, got ", x.scalar_type());
   if (x.dim() < 1 || x.size(-1) != k) refuse("x must have ", k, " columns, got shape ", x.sizes());
-  const Tensor b = bias.value_or(Tensor()), r = residual.value_or(Tensor());
   if (b.defined()) {
     on_gpu("bias", b, dev);
     if (b.scalar_type() != type || b.dim() != 1 || b.size(0) != n) refuse("bias must be (", n, ",) of ", type);
@@ -296,6 +304,7 @@ struct PolicyLossBackward : public Node {
     std::lock_guard<std::mutex> lock(mutex_);
     variable_list out(1);
     if (!grads[0].defined() || !task_should_compute_output(0)) return out;
+    refuse_tangents("the gradient of policy_loss", {&grads[0]});
     const Tensor l0 = logits.unpack(), a0 = action.unpack(), m0 = masked ? mask.unpack() : Tensor(), s0 = save.unpack();
     {
       at::AutoDispatchBelowADInplaceOrView below;
@@ -315,6 +324,8 @@ struct PolicyLossBackward : public Node {
 
 std::pair<Tensor, Tensor> policy_loss(const Tensor& logits, const Tensor& action, const Tensor& old_log_prob, const Tensor& advantage, const MaybeTensor& mask,
                                       const MaybeTensor& ref_log_prob, double lo, double hi, double kl, double ent) {
+  const Tensor ref_or_none = ref_log_prob.value_or(Tensor());
+  refuse_tangents("policy_loss", {&logits, &old_log_prob, &advantage, &ref_or_none});
   check_logits(logits);
   const at::Device dev = logits.device();
   if (!(lo >= 0.0 && lo <= 1.0 && hi >= 0.0)) refuse("clip must be a number in 0..1 or a pair (lo, hi) with lo in 0..1 and hi >= 0");
@@ -365,6 +376,8 @@ std::pair<Tensor, Tensor> policy_loss(const Tensor& logits, const Tensor& action
 // ---- sampling -------------------------------------------------------------------------------------------------------------------------
 
 std::pair<Tensor, Tensor> sample_actions(const Tensor& logits, const MaybeTensor& uniform) {
+  const Tensor uniform_or_none = uniform.value_or(Tensor());
+  refuse_tangents("sample_actions", {&logits, &uniform_or_none});
   check_logits(logits);
   const at::Device dev = logits.device();
   if (logits.requires_grad() && at::GradMode::is_enabled()) refuse("a draw has no gradient: pass logits.detach(), or call it under torch.no_grad()");
@@ -385,6 +398,8 @@ std::pair<Tensor, Tensor> sample_actions(const Tensor& logits, const MaybeTensor
 
 std::tuple<Tensor, Tensor, Tensor> advantages(const Tensor& reward, const Tensor& value, const Tensor& last_value, const Tensor& terminated, const Tensor& truncated, double gamma,
                                               double lam, bool next_step, const MaybeTensor& done, const MaybeTensor& final_value) {
+  const Tensor final_or_none = final_value.value_or(Tensor());
+  refuse_tangents("advantages", {&reward, &value, &last_value, &final_or_none});
   on_gpu("value", value);
   const at::Device dev = value.device();
   const auto type = value.scalar_type();

@@ -40,3 +40,17 @@ def test_policy_loss_backward_in_a_graph_of_its_own(dt):
             backward.replay()
             torch.cuda.synchronize()
             assert torch.equal(d, want[f]), (i, f, spoil)
+
+
+def test_a_tangent_of_the_incoming_gradient_is_refused():
+    """(forward over reverse: the gradient's own tangent would be lost)"""
+    import torch.autograd.forward_ad as fw
+    x, a, old, adv, ref, mask = loss_inputs(40, 7, torch.float32, 3)
+    x = x.contiguous().requires_grad_(True)
+    w = torch.randn((5, 7), generator=gen(1), device="cuda", requires_grad=True)
+    for y in (mg().linear(x, w, activation="tanh"), mg().policy_loss(x, a, old, adv)[0]):
+        with fw.dual_level():
+            g = fw.make_dual(torch.ones_like(y), torch.ones_like(y))
+            with pytest.raises((RuntimeError, ValueError), match="forward-mode"):
+                torch.autograd.grad(y, [x], g, retain_graph=True)
+        torch.autograd.grad(y, [x], torch.ones_like(y))

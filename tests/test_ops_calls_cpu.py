@@ -1,0 +1,36 @@
+"""Calls that the learning operators refuse before they look at anything else, so that no GPU is needed to see it."""
+import pytest
+
+torch = pytest.importorskip("torch")
+
+import minigrid_amd as mg
+
+
+def t(*shape, dtype=torch.float32):
+    return torch.zeros(shape, dtype=dtype)
+
+
+# every floating-point argument of every operator
+TANGENTS = {
+    "linear x": lambda f: mg.linear(f(t(2, 3)), t(4, 3)), "linear weight": lambda f: mg.linear(t(2, 3), f(t(4, 3))),
+    "linear bias": lambda f: mg.linear(t(2, 3), t(4, 3), f(t(4))), "linear residual": lambda f: mg.linear(t(2, 3), t(4, 3), residual=f(t(2, 4))),
+    "loss logits": lambda f: mg.policy_loss(f(t(2, 7)), t(2, dtype=torch.int64), t(2), t(2)),
+    "loss old_log_prob": lambda f: mg.policy_loss(t(2, 7), t(2, dtype=torch.int64), f(t(2)), t(2)),
+    "loss advantage": lambda f: mg.policy_loss(t(2, 7), t(2, dtype=torch.int64), t(2), f(t(2))),
+    "loss ref_log_prob": lambda f: mg.policy_loss(t(2, 7), t(2, dtype=torch.int64), t(2), t(2), ref_log_prob=f(t(2))),
+    "draw logits": lambda f: mg.sample_actions(f(t(2, 7))), "draw uniform": lambda f: mg.sample_actions(t(2, 7), f(t(2))),
+    "advantages reward": lambda f: mg.advantages(f(t(2, 3)), t(2, 3), t(3), t(2, 3).bool(), t(2, 3).bool()),
+    "advantages value": lambda f: mg.advantages(t(2, 3), f(t(2, 3)), t(3), t(2, 3).bool(), t(2, 3).bool()),
+    "advantages last_value": lambda f: mg.advantages(t(2, 3), t(2, 3), f(t(3)), t(2, 3).bool(), t(2, 3).bool()),
+    "advantages final_value": lambda f: mg.advantages(t(2, 3), t(2, 3), t(3), t(2, 3).bool(), t(2, 3).bool(), autoreset_mode="same_step", final_value=f(t(2, 3))),
+}
+
+
+@pytest.mark.parametrize("grad", [True, False])
+@pytest.mark.parametrize("name", list(TANGENTS))
+def test_a_tangent_is_refused(name, grad):
+    """there is no forward-mode derivative: a result without a tangent would be taken for a constant (torch.no_grad() does not turn forward mode off)"""
+    import torch.autograd.forward_ad as fw
+    with fw.dual_level(), torch.set_grad_enabled(grad):
+        with pytest.raises(ValueError, match="forward-mode"):
+            TANGENTS[name](lambda v: fw.make_dual(v, torch.ones_like(v)))
