@@ -7,7 +7,9 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPException.h>
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>
@@ -144,6 +146,13 @@ void refuse_capture_beside_eager(at::Device dev, std::initializer_list<const Ten
   }
 }
 
+// A tracer records the tensors that an operator makes and not what fills them: the traced function would return uninitialised memory.
+void refuse_tracing(const char* name) {
+  typedef c10::impl::TorchDispatchModeTLS Modes;
+  if (torch::jit::tracer::isTracing() || (Modes::any_modes_set() && Modes::get_mode(c10::impl::TorchDispatchModeKey::PROXY)))
+    refuse(name, " cannot be traced: the trace would not hold the operator (a captured graph does)");
+}
+
 // There is no forward-mode derivative: a result without a tangent would be taken for a constant.
 void refuse_tangents(const char* name, std::initializer_list<const Tensor*> inputs) {
   for (const Tensor* t : inputs)
@@ -167,6 +176,7 @@ struct LinearBackward : public Node {
     std::lock_guard<std::mutex> lock(mutex_);
     variable_list out(4);
     if (!grads[0].defined()) return out;
+    refuse_tracing("the gradient of linear");
     refuse_tangents("the gradient of linear", {&grads[0]});
     const Tensor x0 = x.unpack(), w0 = w.unpack(), z0 = act ? z.unpack(shared_from_this()) : Tensor();
     const bool want_x = task_should_compute_output(0), want_w = task_should_compute_output(1), want_b = task_should_compute_output(2);
@@ -211,6 +221,7 @@ struct LinearBackward : public Node {
 
 Tensor linear(const Tensor& x, const Tensor& w, const MaybeTensor& bias, int64_t act, const MaybeTensor& residual) {
   const Tensor b = bias.value_or(Tensor()), r = residual.value_or(Tensor());
+  refuse_tracing("linear");
   refuse_tangents("linear", {&x, &w, &b, &r});
   on_gpu("weight", w);
   const at::Device dev = w.device();
@@ -304,6 +315,7 @@ struct PolicyLossBackward : public Node {
     std::lock_guard<std::mutex> lock(mutex_);
     variable_list out(1);
     if (!grads[0].defined() || !task_should_compute_output(0)) return out;
+    refuse_tracing("the gradient of policy_loss");
     refuse_tangents("the gradient of policy_loss", {&grads[0]});
     const Tensor l0 = logits.unpack(), a0 = action.unpack(), m0 = masked ? mask.unpack() : Tensor(), s0 = save.unpack();
     {
@@ -325,6 +337,7 @@ struct PolicyLossBackward : public Node {
 std::pair<Tensor, Tensor> policy_loss(const Tensor& logits, const Tensor& action, const Tensor& old_log_prob, const Tensor& advantage, const MaybeTensor& mask,
                                       const MaybeTensor& ref_log_prob, double lo, double hi, double kl, double ent) {
   const Tensor ref_or_none = ref_log_prob.value_or(Tensor());
+  refuse_tracing("policy_loss");
   refuse_tangents("policy_loss", {&logits, &old_log_prob, &advantage, &ref_or_none});
   check_logits(logits);
   const at::Device dev = logits.device();
@@ -377,6 +390,7 @@ std::pair<Tensor, Tensor> policy_loss(const Tensor& logits, const Tensor& action
 
 std::pair<Tensor, Tensor> sample_actions(const Tensor& logits, const MaybeTensor& uniform) {
   const Tensor uniform_or_none = uniform.value_or(Tensor());
+  refuse_tracing("sample_actions");
   refuse_tangents("sample_actions", {&logits, &uniform_or_none});
   check_logits(logits);
   const at::Device dev = logits.device();
@@ -399,6 +413,7 @@ std::pair<Tensor, Tensor> sample_actions(const Tensor& logits, const MaybeTensor
 std::tuple<Tensor, Tensor, Tensor> advantages(const Tensor& reward, const Tensor& value, const Tensor& last_value, const Tensor& terminated, const Tensor& truncated, double gamma,
                                               double lam, bool next_step, const MaybeTensor& done, const MaybeTensor& final_value) {
   const Tensor final_or_none = final_value.value_or(Tensor());
+  refuse_tracing("advantages");
   refuse_tangents("advantages", {&reward, &value, &last_value, &final_or_none});
   on_gpu("value", value);
   const at::Device dev = value.device();

@@ -7,7 +7,8 @@
 
 All of them take torch tensors on an MI355X and run hand-written kernels of libminigrid_hip.so (include/minigrid_ops.h) on the tensors' device and its
 current stream, in the manner of torch's own operators: nothing synchronises, results are new tensors, a call may be captured into a graph.  There is no
-CPU fallback, and no forward-mode derivative: an argument that carries a tangent is refused.  What is checked and bound per call is C++ (csrc/ops/mg_torch.cpp).  `MiniGridVecEnv.rollout(policy=...)` and
+CPU fallback, and no forward-mode derivative: an argument that carries a tangent is refused.  So is a
+call that is being traced (torch.jit.trace, make_fx): a trace would hold the result's memory and not what fills it.  What is checked and bound per call is C++ (csrc/ops/mg_torch.cpp).  `MiniGridVecEnv.rollout(policy=...)` and
 `minigrid_amd.policy.ActorCritic` are built from them.
 """
 from __future__ import annotations

@@ -34,3 +34,22 @@ def test_a_tangent_is_refused(name, grad):
     with fw.dual_level(), torch.set_grad_enabled(grad):
         with pytest.raises(ValueError, match="forward-mode"):
             TANGENTS[name](lambda v: fw.make_dual(v, torch.ones_like(v)))
+
+
+CALLS = {
+    "linear": (lambda x: mg.linear(x, t(4, 3)), t(2, 3)), "policy_loss": (lambda x: mg.policy_loss(x, t(2, dtype=torch.int64), t(2), t(2)), t(2, 7)),
+    "sample_actions": (lambda x: mg.sample_actions(x), t(2, 7)), "advantages": (lambda x: mg.advantages(x, x, t(3), t(2, 3).bool(), t(2, 3).bool()), t(2, 3)),
+}
+
+
+@pytest.mark.parametrize("name", list(CALLS))
+def test_a_trace_is_refused(name):
+    """a trace would record the result's allocation and not the operator, and return uninitialised memory"""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    f, x = CALLS[name]
+    with pytest.raises(ValueError, match="traced"):
+        torch.jit.trace(f, (x,))
+    with pytest.raises(ValueError, match="traced"):
+        make_fx(f)(x)
+    with pytest.raises(ValueError, match="no CPU fallback"):         # (not being traced, the call comes as far as its arguments)
+        f(x)
