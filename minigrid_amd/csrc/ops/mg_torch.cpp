@@ -70,6 +70,8 @@ bool is_float(at::ScalarType t) { return t == at::kFloat || t == at::kBFloat16 |
 void on_gpu(const char* name, const Tensor& t) {
   if (!t.is_cuda()) refuse(name, " must be on the GPU: minigrid_amd has no CPU fallback");
   if (t.layout() != at::kStrided) refuse(name, " must be a dense tensor");
+  // (an optional argument without memory would be taken for one that was not given)
+  if (t.numel() && !t.const_data_ptr()) refuse(name, " has no memory: a fake or wrapped tensor cannot be read");
 }
 void on_gpu(const char* name, const Tensor& t, at::Device dev) {
   on_gpu(name, t);

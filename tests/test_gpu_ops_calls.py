@@ -54,3 +54,17 @@ def test_a_tangent_of_the_incoming_gradient_is_refused():
             with pytest.raises((RuntimeError, ValueError), match="forward-mode"):
                 torch.autograd.grad(y, [x], g, retain_graph=True)
         torch.autograd.grad(y, [x], torch.ones_like(y))
+
+
+def test_a_fake_tensor_beside_real_ones_is_refused():
+    """(its address is 0: an optional argument would be taken for one that was not given)"""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    x, w, b, r, dy = linear_inputs(50, 24, 40, torch.float32, False, True, True, False, 5)
+    l, a, old, adv, ref, mask = loss_inputs(40, 7, torch.float32, 3)
+    with FakeTensorMode():
+        fake = lambda t: torch.empty(t.shape, dtype=t.dtype, device="cuda")
+        fb, fr, fref, fmask, fu = fake(b), fake(r), fake(ref), fake(mask), fake(ref)
+    for call in (lambda: mg().linear(x, w, fb), lambda: mg().linear(x, w, residual=fr), lambda: mg().policy_loss(l, a, old, adv, mask=fmask),
+                 lambda: mg().policy_loss(l, a, old, adv, ref_log_prob=fref), lambda: mg().sample_actions(l, fu)):
+        with pytest.raises(ValueError, match="has no memory"):
+            call()

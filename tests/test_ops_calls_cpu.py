@@ -53,3 +53,12 @@ def test_a_trace_is_refused(name):
         make_fx(f)(x)
     with pytest.raises(ValueError, match="no CPU fallback"):         # (not being traced, the call comes as far as its arguments)
         f(x)
+
+
+@pytest.mark.parametrize("name", list(CALLS))
+def test_tensors_without_memory_are_refused(name):
+    """a fake tensor says that it is on the GPU and holds nothing that a kernel could read"""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    f, x = CALLS[name]
+    with FakeTensorMode(), torch.device("cuda"), pytest.raises(ValueError, match="has no memory"):
+        f(torch.empty(x.shape))
