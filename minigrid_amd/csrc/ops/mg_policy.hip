@@ -2,8 +2,9 @@
 //
 // A row's distribution enters through three sums around its largest logit m:  s = sum e^{l - m},  t = sum e^{l - m} (l - m); then log-sum-exp = m + log s,
 // entropy = log s - t / s.  Both are gathered in one pass over the logits, the maximum running along.  What the loss decides by (is the ratio
-// beyond the clipping border?) and what the draw decides by (where does the running sum pass u s?) is held in 64 bits: a value next to a border
-// falls on the side that the mathematics says.
+// beyond the clipping border?) and what the draw decides by (where does the running sum pass u s?) is decided in 64 bits: a value next to a border
+// falls on the side that the mathematics says.  The draw's sums and those of a loss over up to 64 columns are 64-bit throughout; longer rows of a loss
+// are summed from 32-bit exponentials, and a row whose ratio lies within their error of its border is summed again in 64 bits (row_result).
 #include "mg_ops.h"
 
 namespace mgo {
@@ -49,21 +50,22 @@ template <class A> __device__ __forceinline__ int64_t action_of(const A& a, int6
 
 struct Terms { double policy, kl, entropy, clipped, count; };
 
-// the loss terms of a row that counts, from its statistics
-__device__ __forceinline__ Saved row_terms(const LossArgs& a, int64_t i, double lse, double entropy, double chosen, Terms& sum) {
-  const double lp = chosen - lse, adv = a.adv[i], q = exp(lp - (double)a.old_lp[i]);
-  const bool clipped = adv >= 0.0 ? q > a.hi : q < a.lo;
-  const double policy = -(clipped ? (adv >= 0.0 ? a.hi : a.lo) : q) * adv;
+// The loss terms of a row that counts, from its statistics; what its backward pass needs is returned.  error: the ratio is known up to the factor 1 +- error.  Where
+// that leaves open whether it is beyond its border (`open`), nothing is added.  (A border of 0 or infinity leaves nothing open, nor does an error of 0.)
+__device__ __forceinline__ Saved row_terms(const LossArgs& a, int64_t i, double lse, double entropy, double chosen, double error, bool& open, Terms& sum) {
+  const double lp = chosen - lse, adv = a.adv[i], q = exp(lp - (double)a.old_lp[i]), border = adv >= 0.0 ? a.hi : a.lo;
+  open = q > border * (1.0 - error) && q < border * (1.0 + error);
+  if (open) return {};
+  const bool clipped = adv >= 0.0 ? q > border : q < border;
+  const double policy = -(clipped ? border : q) * adv;
   double dlp = clipped ? 0.0 : -q * adv, kl = 0.0;
   if (a.ref_lp) {
     const double gap = (double)a.ref_lp[i] - lp, e = exp(gap);
     kl = e - gap - 1.0;
     dlp += a.kl * (1.0 - e);
   }
-  const Saved k = {lse, (float)dlp, (float)entropy};
-  if (a.save) a.save[i] = k;
   sum.policy += policy; sum.kl += kl; sum.entropy += entropy; sum.clipped += clipped ? 1.0 : 0.0; sum.count += 1.0;
-  return k;
+  return {lse, (float)dlp, (float)entropy};
 }
 
 __device__ __forceinline__ void write_out(const LossArgs& a, const Terms& t, float* out) {
@@ -132,7 +134,9 @@ __global__ void k_loss_small(LossArgs a, double* part, float* out) {
     }
     const double ls = log(s);
     const int64_t act = action_of(a, i);
-    row_terms(a, i, (double)m + ls, ls - t / s, act >= 0 && act < vocab ? (double)l[act] : __builtin_nan(""), sum);
+    bool open;
+    const Saved k = row_terms(a, i, (double)m + ls, ls - t / s, act >= 0 && act < vocab ? (double)l[act] : __builtin_nan(""), 0.0, open, sum);
+    if (a.save) a.save[i] = k;
   }
   // the workgroup's sums; LDS is free again
   wave_sum(sum);
@@ -338,22 +342,51 @@ __global__ __launch_bounds__(1024) void k_count(const uint8_t* mask, int64_t row
   }
 }
 
-// what a row's thread 0 makes of its sums
+// what a row's thread 0 makes of its sums; error and open as in row_terms
 template <class T>
-__device__ __forceinline__ Saved row_result(const LossArgs& a, int64_t i, const T* row, float m, double s, double t, Terms& sum) {
+__device__ __forceinline__ Saved row_result(const LossArgs& a, int64_t i, const T* row, float m, double s, double t, double error, bool& open, Terms& sum) {
   const double ls = log(s);
   const int64_t act = action_of(a, i);
-  return row_terms(a, i, (double)m + ls, ls - t / s, act >= 0 && act < a.vocab ? (double)(float)row[act] : __builtin_nan(""), sum);
+  const Saved k = row_terms(a, i, (double)m + ls, ls - t / s, act >= 0 && act < a.vocab ? (double)(float)row[act] : __builtin_nan(""), error, open, sum);
+  if (a.save && !open) a.save[i] = k;
+  return k;
 }
 
-// (called, not inlined: the constants of its exp and log would be held in registers over the whole loop, next to the row)
+// The sums of a long row are made in 32 bits: d = l - m is rounded (2^-24 |d|), so is d log2 e (2^-24 |d|, and its constant another 1.4e-8 |d|), the exponential is
+// good to 2^-23, and up to eight terms are added in 32 bits (7 x 2^-24).  So s, and with it the ratio, is off by at most 2^-24 (9 + 2.3 D) of itself, D = -t / s
+// the mean of |d| under the row's distribution.  Where that leaves open whether the ratio is beyond its border (a row in 10^5 or so), the row's first wave sums
+// it again with 64-bit exponentials.
+__device__ __forceinline__ double sums_error(double s, double t) { return 0x1p-24 * (16.0 - 4.0 * (t / s)); }
+struct Sums64 { double s, t; };
 template <class T>
-__device__ __noinline__ Saved row_result_call(const LossArgs& a, int64_t i, const T* row, float m, double s, double t, Terms* sum) { return row_result(a, i, row, m, s, t, *sum); }
+__device__ __noinline__ Sums64 wave_sums_64(const T* row, int64_t vocab, float m) {
+  double s = 0.0, t = 0.0;
+#pragma unroll 4
+  for (int64_t c = threadIdx.x; c < vocab; c += 64) {
+    const double d = (double)(float)row[c] - (double)m, e = exp_neg(d);
+    s += e;
+    t += e == 0.0 ? 0.0 : e * d;
+  }
+  return {wave_sum(s), wave_sum(t)};
+}
+
+// By the row's first wave, with arguments and results in LDS.  (Called, not inlined: the constants of its exp and log would be held in registers over the whole
+// loop, next to the row.)
+struct LossShared { LossArgs a; Terms sum; Saved saved; };
+template <class T>
+__device__ __noinline__ void row_result_call(LossShared* sh, int64_t i, const T* row, float m, double s, double t) {
+  bool open = false;
+  if (threadIdx.x == 0) sh->saved = row_result(sh->a, i, row, m, s, t, sums_error(s, t), open, sh->sum);
+  if (!__ballot(open)) return;
+  const Sums64 w = wave_sums_64<T>(row, sh->a.vocab, m);
+  if (threadIdx.x == 0) sh->saved = row_result(sh->a, i, row, m, w.s, w.t, 0.0, open, sh->sum);
+}
 
 // A workgroup per row at a time, every gridDim-th row: rows of up to C x NT 16-byte chunks are held in registers, so the maximum, the sums and, where
-// dlogits is wanted, the gradient (for the factor 1) take one trip to memory.  16 384 x 40 961 bf16, a quarter masked: 2.35 GB in 625 us, 3.8 TB/s, bound by
-// memory and by about twenty vector instructions an element together (two workgroups a CU, 124 registers).  The loss and the gradient from two readings
-// took 719 us, a second reading through the caches 814.
+// dlogits is wanted, the gradient (for the factor 1) take one trip to memory.  16 384 x 40 961 bf16, a quarter masked: 2.35 GB in 517 us, 4.5 TB/s, bound by
+// memory and by about twenty vector instructions an element together (two workgroups a CU, 127 registers).  The loss and the gradient from two readings
+// took 719 us, a second reading through the caches 814.  (Handed to the call per row in scratch memory and not in LDS, the arguments cost 100 us of that, and of
+// 65 536 x 1 000 f32 424 us where it is 282.)
 // count: how many rows count (where dlogits and a mask are there), else all do.
 template <class T, int NT, int C>
 __global__ __launch_bounds__(NT, 4) void k_loss_held(LossArgs a, double* part, const double* count, T* dlogits) {
@@ -361,9 +394,9 @@ __global__ __launch_bounds__(NT, 4) void k_loss_held(LossArgs a, double* part, c
   typedef T VT __attribute__((ext_vector_type(N)));
   __shared__ float wm[W];
   __shared__ double ws[W], wt[W];
-  __shared__ Saved saved;
+  __shared__ LossShared sh;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  Terms sum = {};
+  if (tid == 0) { sh.a = a; sh.sum = {}; }                         // (the first wave reads it behind the first barrier)
   float share = 0.0f;
   if (dlogits) share = 1.0f / (float)(a.mask ? *count : (double)a.rows);
   for (int64_t i = blockIdx.x; i < a.rows; i += gridDim.x) {
@@ -434,14 +467,14 @@ __global__ __launch_bounds__(NT, 4) void k_loss_held(LossArgs a, double* part, c
     t = wave_sum(t);
     if (lane == 0) { ws[wave] = s; wt[wave] = t; }
     __syncthreads();
-    if (tid == 0) {
+    if (tid < 64) {
 #pragma unroll
       for (int w = 1; w < W; w++) { s += ws[w]; t += wt[w]; }
-      saved = row_result_call<T>(a, i, row, m, s, t * LN2, &sum);
+      row_result_call<T>(&sh, i, row, m, s, t * LN2);
     }
-    if (!dlogits) continue;                                      // (thread 0 has read what the next row overwrites before it comes to the next barrier)
+    if (!dlogits) continue;                                      // (the first wave has read what the next row overwrites before it comes to the next barrier)
     __syncthreads();
-    const GradRow g(saved, saved.dlp * share, (float)a.ent * share);
+    const GradRow g(sh.saved, sh.saved.dlp * share, (float)a.ent * share);
     const int act = (int)min((int64_t)0x7fffffff, max((int64_t)-1, action_of(a, i)));
 #pragma unroll
     for (int q = 0; q < C; q++) {
@@ -460,7 +493,7 @@ __global__ __launch_bounds__(NT, 4) void k_loss_held(LossArgs a, double* part, c
       d[at] = x[0];
     }
   }
-  if (tid == 0) put_part(part, gridDim.x, blockIdx.x, sum);
+  if (tid == 0) put_part(part, gridDim.x, blockIdx.x, sh.sum);
 }
 
 // rows that no workgroup's registers hold: their sums alone, the maximum running along
@@ -479,7 +512,13 @@ __global__ __launch_bounds__(256, 4) void k_loss_rows(LossArgs a, double* part) 
     if (threadIdx.x < 64) {
       s = threadIdx.x < 4 ? w[threadIdx.x] : Sums{NEG_INF, 0.0, 0.0};
       wave_join(s);
-      if (threadIdx.x == 0) row_result(a, i, row, s.m, s.s, s.t, sum);
+      for (double error = sums_error(s.s, s.t);; error = 0.0) {
+        bool open = false;
+        if (threadIdx.x == 0) row_result(a, i, row, s.m, s.s, s.t, error, open, sum);
+        if (!__ballot(open)) break;
+        const Sums64 again = wave_sums_64<T>(row, a.vocab, s.m);
+        s.s = again.s; s.t = again.t;
+      }
     }
   }
   if (threadIdx.x == 0) put_part(part, gridDim.x, blockIdx.x, sum);

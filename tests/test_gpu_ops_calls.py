@@ -68,3 +68,34 @@ def test_a_fake_tensor_beside_real_ones_is_refused():
                  lambda: mg().policy_loss(l, a, old, adv, ref_log_prob=fref), lambda: mg().sample_actions(l, fu)):
         with pytest.raises(ValueError, match="has no memory"):
             call()
+
+
+# rows of every way that the loss is computed: a lane, a workgroup that holds the row, a workgroup that walks it
+@pytest.mark.parametrize("dt,vocab", [("f32", 7), ("f32", 65), ("f32", 100), ("f32", 1000), ("f32", 4099), ("f32", 20487), ("f32", 40961), ("bf16", 64), ("bf16", 100), ("bf16", 1023),
+                                      ("bf16", 40961), ("bf16", 90001), ("f16", 300)])
+@pytest.mark.parametrize("upper", [True, False])
+def test_policy_loss_next_to_the_border(dt, vocab, upper):
+    """ratios as close to 1.3 (or 0.8) as f32 log-probabilities allow, on either side: which rows are clipped is what 64 bits say.  (The action's probability is
+    about 0.88, so old_log_prob lies below 0.5, where f32 has steps of 3e-8 and less.)"""
+    rows = 512
+    g = gen(vocab)
+    x = (torch.randn((rows, vocab), generator=g, device="cuda") * 2).to(DT[dt])
+    a = torch.randint(0, vocab, (rows,), generator=g, device="cuda")
+    x.scatter_(1, a[:, None], (x.double().logsumexp(1, keepdim=True) + 2).to(DT[dt]))
+    lp = torch.log_softmax(x.double(), 1).gather(1, a[:, None])[:, 0]
+    border = 1.0 + 0.3 if upper else 1.0 - 0.2
+    old = (lp - math.log(border)).float()
+    away = lp - old.double() - math.log(border)
+    clipped = away > 0 if upper else away < 0
+    sure = away.abs() > 1e-13                                        # (64-bit sums of a row's exponentials agree to a few 1e-16)
+    assert float(away.abs().max()) < 1e-7 and 0.2 < float(clipped.double().mean()) < 0.8
+    adv = torch.full((rows,), 1.0 if upper else -1.0, device="cuda")
+    X = x.clone().requires_grad_(True)
+    loss, stats = mg().policy_loss(X, a, old, adv, clip=(0.2, 0.3))
+    d, = torch.autograd.grad(loss, X)
+    got = ~(d != 0).any(1)
+    assert torch.equal(got[sure], clipped[sure])
+    assert abs(float(stats[3]) * rows - int(got.sum())) < 0.01
+    with torch.no_grad():
+        again, s2 = mg().policy_loss(x, a, old, adv, clip=(0.2, 0.3))
+    assert torch.equal(again, loss) and torch.equal(s2, stats)
