@@ -300,7 +300,8 @@ MG_API int mg_set_state(mg_env* env, const uint8_t* grid, const int32_t* agent);
  * grids as the library holds them (hidden box contents included), agent records, level words (tracked positions, obstacle lists),
  * every env's np_random position, the sentence levels' instruction trees and object identities, the device policy's step counter.
  * mg_state_size bytes; mg_load_state needs a handle created with the same level / grid / batch size (any observation mode) and
- * re-draws the spare episodes from the restored stream positions.  Both synchronise. */
+ * re-draws the spare episodes from the restored stream positions.  Both synchronise.  Bytes 36..39 are the caller's: written as 0 and not read
+ * (minigrid_amd keeps there how far rollouts of a policy have drawn). */
 MG_API int mg_state_size(mg_env* env, int64_t* bytes);
 MG_API int mg_save_state(mg_env* env, void* buf, int64_t bytes);
 MG_API int mg_load_state(mg_env* env, const void* buf, int64_t bytes);

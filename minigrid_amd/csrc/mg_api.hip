@@ -1662,7 +1662,8 @@ int mg_set_state(mg_env* e, const uint8_t* grid, const int32_t* agent) {
 // ---- lossless checkpoint: everything a live handle's future depends on ------------------------------------------------
 // (mg_get_state / mg_set_state exchange the REFERENCE encoding -- Grid.encode() + the agent tuple -- which, like Grid.decode in the
 // reference, cannot carry what a box hides or an instruction tree; this pair carries the library's own state verbatim.)
-struct StateHeader { uint32_t magic, version; int32_t N, CS, W, H, env_kind, sentence; uint32_t t; uint32_t pad; uint64_t env_steps; };
+struct StateHeader { uint32_t magic, version; int32_t N, CS, W, H, env_kind, sentence; uint32_t t; uint32_t caller; uint64_t env_steps; };   // caller: see mg_save_state
+static_assert(offsetof(StateHeader, caller) == 36, "the header promises byte 36");
 constexpr uint32_t STATE_MAGIC = 0x5453474Du;   // "MGST"
 static size_t state_bytes(const mg_env* e) {
   const size_t N = (size_t)e->N;

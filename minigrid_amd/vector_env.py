@@ -48,6 +48,23 @@ class _DeviceArray:
         self._owner = owner  # keep the env alive
 
 
+_STATE_CALLER = 36                   # byte of a checkpoint that holds the caller's own number (mg_save_state), u32
+
+
+def _draw_seed(seed: int, step: int, base: int) -> int:
+    """The seed of the draws of a rollout that begins `step` steps behind a reset(seed=...): `seed` itself for the first one of a batch that starts at env 0,
+    else the three of them hashed (the finaliser of splitmix64: Steele, Lea and Flood, 2014)."""
+    if step == 0 and base == 0:
+        return seed
+    m, h = (1 << 64) - 1, 0
+    for v in (seed, step, base):
+        h = (h ^ (v & m)) + 0x9E3779B97F4A7C15 & m
+        h = (h ^ h >> 30) * 0xBF58476D1CE4E5B9 & m
+        h = (h ^ h >> 27) * 0x94D049BB133111EB & m
+        h ^= h >> 31
+    return h
+
+
 class MiniGridVecEnv(_VectorEnvBase):
     metadata = {"render_modes": [], "autoreset_mode": "next_step"}
 
@@ -169,6 +186,7 @@ class MiniGridVecEnv(_VectorEnvBase):
         self.width, self.height, self.max_steps = s.width, s.height, s.max_steps
         self._missions = np.asarray(s.missions)
         self._seeded = False
+        self._draws = 0              # steps that rollouts of a policy have drawn actions for since the last reset(seed=...)
         self._bind_outputs()
 
     def _bind_outputs(self):
@@ -360,6 +378,8 @@ class MiniGridVecEnv(_VectorEnvBase):
         rc = self._lib.mg_reset(self._h, None if seeds is None else self._p(np.ascontiguousarray(seeds)),
                                 None if mask is None else self._p(mask))
         B.check(rc, self._h)
+        if seed is not None and mask is None:
+            self._draws = 0
         obs, _, _, _ = self._collect()
         return obs, {}
 
@@ -447,8 +467,10 @@ class MiniGridVecEnv(_VectorEnvBase):
         LDS; step j writes trajectory slot (steps-1-j) % traj_slots, so slot 0 is the last step.
 
         policy: a callable that takes an observation as `step` returns it and gives (logits (num_envs, 7), value (num_envs,)) --
-        minigrid_amd.policy.ActorCritic, or any other.  The actions are then drawn from its logits (`sample_actions`; action_seed seeds the draws), one
-        launch per step, and the transitions come back as a minigrid_amd.policy.Trajectory.  Needs output="torch"; no gradient is recorded."""
+        minigrid_amd.policy.ActorCritic, or any other.  The actions are then drawn from its logits (`sample_actions`), one launch per step, and the
+        transitions come back as a minigrid_amd.policy.Trajectory.  action_seed seeds the draws, which go on from rollout to rollout: they follow from the seed,
+        the number of steps rolled out since the last reset(seed=...) of all envs (a checkpoint carries it) and env_index_base.  Needs output="torch"; no
+        gradient is recorded."""
         if policy is not None:
             return self._rollout_policy(int(steps), int(action_seed), bool(fused), policy)
         self._no_fused_with_final_obs()
@@ -483,7 +505,8 @@ class MiniGridVecEnv(_VectorEnvBase):
             action = torch.empty((steps, n), dtype=torch.uint8, device=dev)
             log_prob = torch.empty((steps, n), dtype=torch.float32, device=dev)
             value = torch.empty((steps, n), dtype=torch.float32, device=dev)
-            u = torch.rand((steps, n), generator=torch.Generator(dev).manual_seed(action_seed), device=dev)
+            u = torch.rand((steps, n), generator=torch.Generator(dev).manual_seed(_draw_seed(action_seed, self._draws, self.env_index_base)), device=dev)
+            self._draws += steps
             done = (out["terminated"] | out["truncated"]).bool()
             obs = self._collect()[0]
             for t in range(steps):
@@ -609,17 +632,19 @@ class MiniGridVecEnv(_VectorEnvBase):
 
     def save_state(self) -> bytes:
         """Lossless checkpoint of the live batch (mg_save_state): grids incl. what boxes hide, agent records, level words, every env's
-        np_random position, the sentence levels' instruction trees -- what pickling a reference env carries."""
+        np_random position, the sentence levels' instruction trees, how far rollouts of a policy have drawn -- what pickling a reference env carries."""
         nb = C.c_int64()
         B.check(self._lib.mg_state_size(self._h, C.byref(nb)), self._h)
         buf = np.empty(int(nb.value), np.uint8)
         B.check(self._lib.mg_save_state(self._h, self._p(buf), nb), self._h)
+        buf[_STATE_CALLER:_STATE_CALLER + 4].view(np.uint32)[0] = self._draws & 0xffffffff
         return buf.tobytes()
 
     def load_state(self, blob: bytes):
         """Continue from a checkpoint taken from an env of the same level, grid and batch size (any observation configuration)."""
         buf = np.frombuffer(blob, np.uint8).copy()
         B.check(self._lib.mg_load_state(self._h, self._p(buf), C.c_int64(buf.size)), self._h)
+        self._draws = int(buf[_STATE_CALLER:_STATE_CALLER + 4].view(np.uint32)[0])
         self._seeded = True
 
     def __getstate__(self):

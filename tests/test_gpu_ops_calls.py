@@ -99,3 +99,53 @@ def test_policy_loss_next_to_the_border(dt, vocab, upper):
     with torch.no_grad():
         again, s2 = mg().policy_loss(x, a, old, adv, clip=(0.2, 0.3))
     assert torch.equal(again, loss) and torch.equal(s2, stats)
+
+
+def toy_policy(obs):
+    """equal logits; the value is a whole number of the observation, so that it does not depend on how it is summed"""
+    image = obs["image"]
+    n = image.shape[0]
+    return torch.zeros((n, 7), device=image.device), image.reshape(n, -1).sum(1).float() + obs["direction"].float()
+
+
+def toy_envs(n=64, env_id="MiniGrid-Empty-5x5-v0", **kw):
+    return mg().make_vec(env_id, n, output="torch", **kw)
+
+
+def test_rollouts_one_after_the_other_draw_other_numbers():
+    """the draws of a seed go on from rollout to rollout, begin again with reset(seed=...), and are others for other environments and other seeds"""
+    envs = toy_envs()
+    envs.reset(seed=1)
+    a, b, c = (envs.rollout(20, policy=toy_policy).action for _ in range(3))
+    assert not torch.equal(a, b) and not torch.equal(b, c) and not torch.equal(a, c)
+    for e in range(0, 64, 7):                                        # no environment is given the same number at the same step again and again
+        assert not torch.equal(a[:, e], b[:, e])
+    envs.reset(seed=1)
+    again = [envs.rollout(20, policy=toy_policy).action for _ in range(2)]
+    assert torch.equal(a, again[0]) and torch.equal(b, again[1])
+    envs.reset()                                                     # (goes on)
+    assert not torch.equal(envs.rollout(20, policy=toy_policy).action, a)
+    envs.reset(seed=1, options={"reset_mask": [1] + [0] * 63})       # (one environment's map, not the draws of all)
+    assert not torch.equal(envs.rollout(20, policy=toy_policy).action, a)
+    envs.reset(seed=1)
+    assert not torch.equal(envs.rollout(20, action_seed=1, policy=toy_policy).action, a)
+    other = toy_envs(env_index_base=64)
+    other.reset(seed=1)
+    assert not torch.equal(other.rollout(20, policy=toy_policy).action, a)
+    share = torch.bincount(torch.cat([a, b, c]).flatten().long(), minlength=7).double() / (60 * 64)
+    within(share, torch.full((7,), 1 / 7, dtype=torch.float64, device="cuda"), 5 * math.sqrt(6 / 49 / (60 * 64)), "share")
+    envs.close()
+    other.close()
+
+
+def test_a_pickled_env_goes_on_drawing():
+    envs = toy_envs()
+    envs.reset(seed=1)
+    a = envs.rollout(20, policy=toy_policy).action
+    twin, fresh = pickle.loads(pickle.dumps(envs)), toy_envs()
+    fresh.load_state(envs.save_state())
+    want = envs.rollout(20, policy=toy_policy).action
+    assert not torch.equal(want, a)
+    assert torch.equal(twin.rollout(20, policy=toy_policy).action, want) and torch.equal(fresh.rollout(20, policy=toy_policy).action, want)
+    for e in (envs, twin, fresh):
+        e.close()
