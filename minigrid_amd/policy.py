@@ -53,12 +53,14 @@ class Trajectory:
     done: torch.Tensor
     last_value: torch.Tensor
     autoreset_mode: str
+    final_value: Optional[torch.Tensor] = None
 
     def advantages(self, gamma: float = 0.99, lam: float = 0.95):
-        """(advantage, return, valid) of the rollout: `ops.advantages`"""
+        """(advantage, return, valid) of the rollout: `ops.advantages`.  In the same_step mode a truncated step is bootstrapped from final_value, and counts as worth
+        0 without it."""
         next_step = self.autoreset_mode == "next_step"
         return ops.advantages(self.reward, self.value, self.last_value, self.terminated, self.truncated, gamma=gamma, lam=lam,
-                              autoreset_mode=self.autoreset_mode, done=self.done if next_step else None)
+                              autoreset_mode=self.autoreset_mode, done=self.done if next_step else None, final_value=None if next_step else self.final_value)
 
     def loss(self, logits, advantage, mask=None, *, index: Optional[torch.Tensor] = None, ref_log_prob=None, **kw):
         """`ops.policy_loss` of new logits for all transitions, or for those at `index` of the flattened (steps x envs) -- a minibatch; advantage, mask and

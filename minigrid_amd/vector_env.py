@@ -422,7 +422,8 @@ class MiniGridVecEnv(_VectorEnvBase):
             if not bool(done.any()):
                 return obs, rew, term, trunc, {}
             # the outputs are views of trajectory slot 0, which the reset launch rewrites: keep what this step reported
-            rew, term, trunc = rew.clone(), term.clone(), trunc.clone()
+            if rew is not None:
+                rew, term, trunc = rew.clone(), term.clone(), trunc.clone()
             if want_final:
                 idx = torch.nonzero(done).flatten()
                 final = obs[idx].clone() if self.image_only else {k: v[idx].clone() for k, v in obs.items()}
@@ -461,7 +462,7 @@ class MiniGridVecEnv(_VectorEnvBase):
             raise ValueError("final_obs=True reports terminal observations from step(), one launch at a time; "
                              "the fused entry points need autoreset_mode='same_step' without it (or 'next_step')")
 
-    def rollout(self, steps: int, action_seed: int = 0, fused: bool = False, policy=None):
+    def rollout(self, steps: int, action_seed: int = 0, fused: bool = False, policy=None, final_value: bool = False):
         """`steps` lockstep steps under a uniform-random policy generated on the device (the loop of
         minigrid/benchmark.py:36-43).  fused: up to `max_fused_steps` steps per kernel launch, the grids resident in
         LDS; step j writes trajectory slot (steps-1-j) % traj_slots, so slot 0 is the last step.
@@ -470,13 +471,20 @@ class MiniGridVecEnv(_VectorEnvBase):
         minigrid_amd.policy.ActorCritic, or any other.  The actions are then drawn from its logits (`sample_actions`), one launch per step, and the
         transitions come back as a minigrid_amd.policy.Trajectory.  action_seed seeds the draws, which go on from rollout to rollout: they follow from the seed,
         the number of steps rolled out since the last reset(seed=...) of all envs (a checkpoint carries it) and env_index_base.  Needs output="torch"; no
-        gradient is recorded."""
+        gradient is recorded.
+
+        final_value (autoreset_mode="same_step" with final_obs=True): the policy is also asked for the value of the observations that truncated steps ended on
+        (Trajectory.final_value; a second launch and a host round trip in steps that end an episode).  Without it the trajectory of a same_step env takes them to
+        be worth 0, as if the episode had been over: its advantages are off by gamma times that value at each truncation, which the call warns of.  In the
+        next_step mode the rows themselves hold these values."""
         if policy is not None:
-            return self._rollout_policy(int(steps), int(action_seed), bool(fused), policy)
+            return self._rollout_policy(int(steps), int(action_seed), bool(fused), policy, bool(final_value))
+        if final_value:
+            raise ValueError("final_value belongs to the rollout of a policy")
         self._no_fused_with_final_obs()
         B.check(self._lib.mg_rollout(self._h, int(steps), int(action_seed), int(fused)), self._h)
 
-    def _rollout_policy(self, steps, action_seed, fused, policy):
+    def _rollout_policy(self, steps, action_seed, fused, policy, final_value):
         if self.output != "torch":
             raise ValueError("rollout(policy=...) needs an env made with output='torch'")
         if fused:
@@ -486,7 +494,15 @@ class MiniGridVecEnv(_VectorEnvBase):
         mode = self.metadata["autoreset_mode"]
         if mode == "disabled":
             raise ValueError("rollout(policy=...) needs an autoreset: autoreset_mode 'next_step' or 'same_step'")
-        self._no_fused_with_final_obs()
+        if final_value and not self._final_obs:
+            raise ValueError("final_value=True needs an env made with autoreset_mode='same_step' and final_obs=True")
+        if self._final_obs and not final_value:
+            raise ValueError("an env made with final_obs=True rolls out a policy with final_value=True")
+        if not final_value:
+            self._no_fused_with_final_obs()
+            if mode == "same_step":
+                import warnings
+                warnings.warn("truncated steps will count as worth 0: make the env with final_obs=True and pass final_value=True for the values of their last observations", stacklevel=3)
         import torch
 
         from .ops import sample_actions
@@ -505,6 +521,7 @@ class MiniGridVecEnv(_VectorEnvBase):
             action = torch.empty((steps, n), dtype=torch.uint8, device=dev)
             log_prob = torch.empty((steps, n), dtype=torch.float32, device=dev)
             value = torch.empty((steps, n), dtype=torch.float32, device=dev)
+            final = torch.zeros((steps, n), dtype=torch.float32, device=dev) if final_value else None
             u = torch.rand((steps, n), generator=torch.Generator(dev).manual_seed(_draw_seed(action_seed, self._draws, self.env_index_base)), device=dev)
             self._draws += steps
             done = (out["terminated"] | out["truncated"]).bool()
@@ -521,13 +538,17 @@ class MiniGridVecEnv(_VectorEnvBase):
                 value[t].copy_(v)
                 B.check(self._lib.mg_step(self._h, C.c_void_p(action[t].data_ptr()), B.ACT_U8, 1), self._h)
                 rec[t].copy_(now)
-                obs = self._collect()[0]
+                obs, _, term, trunc = self._collect()
+                if final_value:
+                    if bool(trunc.any()):                # (the step kernel has left the terminal observations in obs: see __init__)
+                        final[t].copy_(torch.where(trunc, policy(obs)[1].float(), final[t]))
+                    obs = self._same_step_with_final_obs(obs, None, term, trunc, want_final=False)[0]
             last = policy(obs)[1].float().clone()
         field = lambda r, name: r[:, :, lay[name] - at]
         return Trajectory(image=image, direction=field(before, "direction"),
                           mission_id=before.view(torch.int16)[:, :, (lay["mission_id"] - at) // 2], action=action, log_prob=log_prob, value=value,
                           reward=rec.view(torch.float64)[:, :, 0], terminated=field(rec, "terminated"), truncated=field(rec, "truncated"), done=done,
-                          last_value=last, autoreset_mode=mode)
+                          last_value=last, autoreset_mode=mode, final_value=final)
 
     def rollout_block(self, steps: int, action_seed: int = 0, slot0: Optional[int] = None):
         """ONE fused launch of `steps` <= max_fused_steps steps of the device policy; step j lands in trajectory slot slot0 - j

@@ -149,3 +149,60 @@ def test_a_pickled_env_goes_on_drawing():
     assert torch.equal(twin.rollout(20, policy=toy_policy).action, want) and torch.equal(fresh.rollout(20, policy=toy_policy).action, want)
     for e in (envs, twin, fresh):
         e.close()
+
+
+@pytest.mark.parametrize("env_id", ["MiniGrid-DoorKey-5x5-v0", "BabyAI-GoToRedBall-v0", "MiniGrid-Dynamic-Obstacles-5x5-v0"])
+def test_truncated_steps_are_worth_the_observation_they_ended_on(env_id):
+    """same_step with final_obs=True and final_value=True: the policy's value of every terminal observation comes with the trajectory, and its advantages use it"""
+    n, steps = 96, 60
+    envs, twin = (toy_envs(n, env_id, autoreset_mode="same_step", final_obs=True, max_steps=9) for _ in range(2))
+    envs.reset(seed=5)
+    obs, _ = twin.reset(seed=5)
+    traj = envs.rollout(steps, action_seed=3, policy=toy_policy, final_value=True)
+    final = torch.zeros((steps, n), device="cuda")
+    for i in range(steps):                                           # the same environments stepped by hand with the drawn actions
+        assert torch.equal(traj.image[i], obs["image"]) and torch.equal(traj.direction[i], obs["direction"]) and torch.equal(traj.mission_id[i], obs["mission_id"])
+        assert torch.equal(traj.value[i], toy_policy(obs)[1])
+        obs, rew, term, trunc, info = twin.step(traj.action[i])
+        assert torch.equal(traj.reward[i], rew) and torch.equal(traj.terminated[i].bool(), term) and torch.equal(traj.truncated[i].bool(), trunc)
+        if info:
+            final[i, info["final_obs_indices"]] = toy_policy(info["final_obs"])[1]
+    assert torch.equal(traj.last_value, toy_policy(obs)[1])
+    cut = traj.truncated.bool()
+    assert int(cut.sum()) > n and torch.equal(traj.final_value[cut], final[cut]) and bool((final[cut] > 0).all())
+    adv, ret, valid = traj.advantages(0.97, 0.9)
+    args = (traj.reward, traj.value, traj.last_value, traj.terminated, traj.truncated, 0.97, 0.9, "same_step")
+    wa, wr, wv = advantages64(*args, None, final)
+    assert torch.equal(valid, wv) and bool(valid.all())
+    within(adv, wa, 1.01 * U * wa.abs() + 1e-12, "advantage")
+    within(ret, wr, 1.01 * U * wr.abs() + 1e-12, "return")
+    assert float((wa - advantages64(*args, None, None)[0]).abs().max()) > 1.0                 # (worth 0 otherwise: that is far off here)
+    # a second rollout goes on where the first ended
+    more = envs.rollout(3, action_seed=4, policy=toy_policy, final_value=True)
+    assert torch.equal(more.image[0], obs["image"])
+    envs.close()
+    twin.close()
+
+
+def test_final_values_where_there_are_none_are_refused():
+    for kw in (dict(), dict(autoreset_mode="same_step")):
+        envs = toy_envs(8, **kw)
+        envs.reset(seed=0)
+        with pytest.raises(ValueError, match="final_obs=True"):
+            envs.rollout(4, policy=toy_policy, final_value=True)
+        envs.close()
+    envs = toy_envs(8, autoreset_mode="same_step", final_obs=True)
+    with pytest.raises(ValueError, match="final_value=True"):
+        envs.rollout(4, policy=toy_policy)
+    with pytest.raises(ValueError, match="policy"):
+        envs.rollout(4, final_value=True)
+    envs.close()
+
+
+def test_a_rollout_that_leaves_truncated_steps_worth_nothing_says_so():
+    envs = toy_envs(8, autoreset_mode="same_step")
+    envs.reset(seed=0)
+    with pytest.warns(UserWarning, match="final_value=True"):
+        traj = envs.rollout(4, policy=toy_policy)
+    assert traj.final_value is None
+    envs.close()
