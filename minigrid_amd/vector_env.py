@@ -186,6 +186,9 @@ class MiniGridVecEnv(_VectorEnvBase):
         self.width, self.height, self.max_steps = s.width, s.height, s.max_steps
         self._missions = np.asarray(s.missions)
         self._seeded = False
+        # what trajectory slot 0 holds: "step" (of the last step: its observation and its flags; of a full reset: no flags are due), "observed" (the live observation,
+        # the flags cleared), "stale" (something else)
+        self._slot0 = "step"
         self._draws = 0              # steps that rollouts of a policy have drawn actions for since the last reset(seed=...)
         self._bind_outputs()
 
@@ -380,6 +383,7 @@ class MiniGridVecEnv(_VectorEnvBase):
         B.check(rc, self._h)
         if seed is not None and mask is None:
             self._draws = 0
+        self._slot0 = "step" if mask is None else "observed"
         obs, _, _, _ = self._collect()
         return obs, {}
 
@@ -404,6 +408,7 @@ class MiniGridVecEnv(_VectorEnvBase):
             self._last_actions = a          # the async H2D copy may still read it after this call returns
             rc = self._lib.mg_step(self._h, self._p(a), dt, 0)
         B.check(rc, self._h)
+        self._slot0 = "step"
         obs, rew, term, trunc = self._collect()
         if self._final_obs:
             return self._same_step_with_final_obs(obs, rew, term, trunc)
@@ -483,6 +488,8 @@ class MiniGridVecEnv(_VectorEnvBase):
             raise ValueError("final_value belongs to the rollout of a policy")
         self._no_fused_with_final_obs()
         B.check(self._lib.mg_rollout(self._h, int(steps), int(action_seed), int(fused)), self._h)
+        if steps:
+            self._slot0 = "step"
 
     def _rollout_policy(self, steps, action_seed, fused, policy, final_value):
         if self.output != "torch":
@@ -524,7 +531,16 @@ class MiniGridVecEnv(_VectorEnvBase):
             final = torch.zeros((steps, n), dtype=torch.float32, device=dev) if final_value else None
             u = torch.rand((steps, n), generator=torch.Generator(dev).manual_seed(_draw_seed(action_seed, self._draws, self.env_index_base)), device=dev)
             self._draws += steps
-            done = (out["terminated"] | out["truncated"]).bool()
+            done = None
+            if self._slot0 != "step":
+                done = torch.from_numpy(self.get_state()[1][:, 6] != 0)                   # (whose reset is due)
+                if self._slot0 == "stale":
+                    if self.spec_row.env_kind == ENV_DYNOBS and bool(done.any()):
+                        raise ValueError("an env whose reset is due cannot be observed without taking it in this level: step() or reset() first")
+                    # (a reset of no env observes all of them as they are)
+                    B.check(self._lib.mg_reset(self._h, None, self._p(np.zeros(n, np.uint8))), self._h)
+            done = (out["terminated"] | out["truncated"]).bool() if done is None or mode != "next_step" else done.to(dev)
+            self._slot0 = "step"
             obs = self._collect()[0]
             for t in range(steps):
                 image[t].copy_(out["image"])
@@ -554,7 +570,9 @@ class MiniGridVecEnv(_VectorEnvBase):
         """ONE fused launch of `steps` <= max_fused_steps steps of the device policy; step j lands in trajectory slot slot0 - j
         (default slot0 = steps - 1), so the launch's step records are the contiguous slots [slot0 - steps + 1, slot0]."""
         self._no_fused_with_final_obs()
-        B.check(self._lib.mg_rollout_block(self._h, int(steps), int(action_seed), int(steps - 1 if slot0 is None else slot0)), self._h)
+        slot0 = int(steps - 1 if slot0 is None else slot0)
+        B.check(self._lib.mg_rollout_block(self._h, int(steps), int(action_seed), slot0), self._h)
+        self._slot0 = "step" if slot0 == steps - 1 else "stale"
 
     def block_view(self, slot_lo: int, nslots: int):
         """Zero-copy torch view of `nslots` consecutive trajectory slots starting at slot_lo: (nslots, slot_bytes) uint8."""
@@ -584,9 +602,13 @@ class MiniGridVecEnv(_VectorEnvBase):
             self._last_actions = a
             rc = self._lib.mg_step_many(self._h, self._p(a), int(a.shape[0]), 0)
             B.check(rc, self._h)
+            if len(a):
+                self._slot0 = "step"
             self.sync()                    # the staged host buffer is reused chunk by chunk
             return
         B.check(rc, self._h)
+        if len(a):
+            self._slot0 = "step"
 
     def _reconfigure(self, **changes):
         """Apply an observation wrapper to THIS env, the way the reference's wrappers wrap the same env object (wrappers.py:187-214):
@@ -617,6 +639,7 @@ class MiniGridVecEnv(_VectorEnvBase):
             if v > 15:
                 raise ValueError("agent_view_size up to 15 is supported on the accelerated path")
         B.check(self._lib.mg_set_obs_config(self._h, C.byref(cfg)), self._h)
+        self._slot0 = "stale"
         self._cfg = cfg
         for k, v in changes.items():
             setattr(self, {"no_death_types": "no_death_types"}.get(k, k), tuple(v) if k == "no_death_types" else v)
@@ -650,6 +673,7 @@ class MiniGridVecEnv(_VectorEnvBase):
         if grid.shape != (self.num_envs, self.width, self.height, 3) or agent.shape != (self.num_envs, 8):
             raise ValueError("bad state shapes")
         B.check(self._lib.mg_set_state(self._h, self._p(grid), self._p(agent)), self._h)
+        self._slot0 = "stale"
 
     def save_state(self) -> bytes:
         """Lossless checkpoint of the live batch (mg_save_state): grids incl. what boxes hide, agent records, level words, every env's
@@ -665,6 +689,7 @@ class MiniGridVecEnv(_VectorEnvBase):
         """Continue from a checkpoint taken from an env of the same level, grid and batch size (any observation configuration)."""
         buf = np.frombuffer(blob, np.uint8).copy()
         B.check(self._lib.mg_load_state(self._h, self._p(buf), C.c_int64(buf.size)), self._h)
+        self._slot0 = "stale"
         self._draws = int(buf[_STATE_CALLER:_STATE_CALLER + 4].view(np.uint32)[0])
         self._seeded = True
 

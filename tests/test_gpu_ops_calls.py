@@ -206,3 +206,80 @@ def test_a_rollout_that_leaves_truncated_steps_worth_nothing_says_so():
         traj = envs.rollout(4, policy=toy_policy)
     assert traj.final_value is None
     envs.close()
+
+
+def step_until_some_end(envs):
+    for _ in range(2000):
+        obs, _, term, trunc, _ = envs.step(torch.full((envs.num_envs,), 2, dtype=torch.uint8, device="cuda"))
+        if bool((term | trunc).any()):
+            return obs, (term | trunc).clone()
+    raise AssertionError("no episode ended")
+
+
+@pytest.mark.parametrize("env_id", ["MiniGrid-DoorKey-5x5-v0", "BabyAI-GoToRedBall-v0", "BabyAI-GoToSeqS5R2-v0"])
+def test_rollout_begins_where_the_env_is(env_id):
+    """behind a restored checkpoint and behind a masked reset the first observation is the live one, and a step that only resets is known as one"""
+    n = 48
+    envs = toy_envs(n, env_id, max_steps=6)
+    envs.reset(seed=3)
+    obs, ended = step_until_some_end(envs)
+    image = obs["image"].clone()
+    twin = toy_envs(n, env_id, max_steps=6)
+    twin.reset(seed=9)
+    twin.load_state(envs.save_state())
+    pickled = pickle.loads(pickle.dumps(envs))
+    want = envs.rollout(9, policy=toy_policy)
+    assert torch.equal(want.done, ended) and torch.equal(want.image[0], image)
+    for e in (twin, pickled):
+        got = e.rollout(9, policy=toy_policy)
+        for name in ("image", "direction", "mission_id", "action", "value", "reward", "terminated", "truncated", "done", "last_value"):
+            assert torch.equal(getattr(got, name), getattr(want, name)), name
+        e.close()
+    # a masked reset: the others are still due for theirs
+    envs.reset(seed=3)
+    obs, ended = step_until_some_end(envs)
+    some = [i % 3 == 0 for i in range(n)]
+    envs.reset(options={"reset_mask": some})
+    done = ended & ~torch.tensor(some, device="cuda")
+    traj = envs.rollout(3, policy=toy_policy)
+    assert torch.equal(traj.done, done) and torch.equal(traj.advantages()[2][0], ~done)
+    envs.close()
+
+
+def test_rollout_of_restored_obstacles():
+    """DynamicObstacles draws its resets when it is observed: a restored env whose reset is due is refused, any other goes on as it would have"""
+    n = 48
+    envs, twin = (toy_envs(n, "MiniGrid-Dynamic-Obstacles-5x5-v0", max_steps=6) for _ in range(2))
+    envs.reset(seed=3)
+    step = lambda: envs.step(torch.zeros(n, dtype=torch.uint8, device="cuda"))
+    while True:
+        _, _, term, trunc, _ = step()
+        if not bool((term | trunc).any()):
+            break
+    twin.reset(seed=9)
+    twin.load_state(envs.save_state())
+    want, got = envs.rollout(9, policy=toy_policy), twin.rollout(9, policy=toy_policy)
+    for name in ("image", "direction", "mission_id", "action", "value", "reward", "terminated", "truncated", "done", "last_value"):
+        assert torch.equal(getattr(got, name), getattr(want, name)), name
+    while True:
+        _, _, term, trunc, _ = step()
+        if bool((term | trunc).any()):
+            break
+    twin.load_state(envs.save_state())
+    with pytest.raises(ValueError, match="reset is due"):
+        twin.rollout(9, policy=toy_policy)
+    twin.step(torch.zeros(n, dtype=torch.uint8, device="cuda"))
+    twin.rollout(2, policy=toy_policy)
+    envs.close()
+    twin.close()
+
+
+def test_rollout_behind_fused_steps():
+    """(a block of fused steps need not leave its last step in slot 0)"""
+    envs = toy_envs(48, "MiniGrid-Empty-5x5-v0", max_steps=20, traj_slots=16)
+    envs.reset(seed=3)
+    envs.rollout_block(4, 0, slot0=11)
+    image, done = envs.torch_outputs(8)["image"].clone(), (envs.torch_outputs(8)["terminated"] | envs.torch_outputs(8)["truncated"]).bool()
+    traj = envs.rollout(3, policy=toy_policy)
+    assert torch.equal(traj.image[0], image) and torch.equal(traj.done, done)
+    envs.close()
