@@ -650,7 +650,11 @@ struct DirectLoader {
   // pass q of the tile at LDS byte address lds (uniform, like the wave's number)
   __device__ __forceinline__ void load(int q, uint32_t lds, int wave) {
     const uint32_t at = lds + q * (THREADS * 16) + wave * 1024;
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(off[COLS ? q & 1 : 0]), "s"(base + q * pass) : "memory");
+    // (m0 is named so that nothing of the compiler's is expected to outlive the statement in it; it warns that it saves no such register for us, which nothing asks for)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(off[COLS ? q & 1 : 0]), "s"(base + q * pass) : "memory", "m0");
+#pragma clang diagnostic pop
   }
   __device__ __forceinline__ void advance() { base += step; }
 };

@@ -62,3 +62,23 @@ def test_tensors_without_memory_are_refused(name):
     f, x = CALLS[name]
     with FakeTensorMode(), torch.device("cuda"), pytest.raises(ValueError, match="has no memory"):
         f(torch.empty(x.shape))
+
+
+def test_assembly_names_the_special_registers_that_it_writes():
+    """a register that an asm statement writes and does not name may hold a value of the compiler's: m0 (the LDS address of a load into LDS) among them"""
+    import glob
+    import os
+    import re
+
+    from conftest import ROOT
+    found = 0
+    for path in glob.glob(os.path.join(ROOT, "minigrid_amd", "csrc", "ops", "*")):
+        if not path.endswith((".h", ".hip", ".inc")):
+            continue
+        for m in re.finditer(r"\basm\s+volatile\s*\((.*?)\);", open(path).read(), re.S):
+            text = m.group(1)
+            for reg in ("m0", "vcc", "scc", "exec"):
+                if re.search(r"\bs_mov_b\d+ +%s\b" % reg, text):
+                    found += 1
+                    assert '"%s"' % reg in text.split(":")[-1], (os.path.basename(path), text)
+    assert found
