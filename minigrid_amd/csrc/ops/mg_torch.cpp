@@ -98,10 +98,30 @@ Tensor matrix(const Tensor& t, int64_t cols) {
 }
 int64_t row_stride(const Tensor& m) { return std::max(m.stride(0), m.size(1)); }     // (the stride of a single row means nothing)
 
-// what the backward pass reads again: the tensor itself where the operator read its memory (a change in place is then noticed), else the copy
-SavedVariable keep(const Tensor& original, const Tensor& used) {
-  return SavedVariable(original.defined() && used.defined() && original.data_ptr() == used.data_ptr() ? original : used, false);
-}
+// What the backward pass reads again.  A saved-tensor hook may hand back another tensor than it was given: one of another type, shape or device would be read out of
+// its bounds, and is refused; strides are looked at again.
+struct Kept {
+  SavedVariable saved;
+  at::ScalarType type = at::kFloat;
+  at::DimVector sizes;
+  at::Device dev = at::kCPU;
+  void put(const Tensor& t, bool is_output = false) {
+    saved = SavedVariable(t, is_output);
+    type = t.scalar_type();
+    sizes = at::DimVector(t.sizes());
+    dev = t.device();
+  }
+  // the tensor itself where the operator read its memory (a change in place is then noticed), else the copy
+  void put(const Tensor& original, const Tensor& used) { put(original.data_ptr() == used.data_ptr() ? original : used); }
+  Tensor get(const char* name, std::shared_ptr<Node> owner = nullptr) const {
+    const Tensor t = saved.unpack(std::move(owner));
+    TORCH_CHECK(t.defined() && t.scalar_type() == type && t.sizes() == at::IntArrayRef(sizes) && t.device() == dev && t.layout() == at::kStrided, name, " was saved as ", type, " ",
+                at::IntArrayRef(sizes), " on ", dev, ", and a saved-tensor hook gave back another type, shape or device");
+    return t;
+  }
+  Tensor get_contiguous(const char* name, std::shared_ptr<Node> owner = nullptr) const { return get(name, std::move(owner)).contiguous(); }
+  void reset_data() { saved.reset_data(); }
+};
 
 at::DimVector with_last(at::IntArrayRef lead, int64_t last) {
   at::DimVector s(lead.begin(), lead.end() - 1);
@@ -164,7 +184,7 @@ void refuse_tangents(const char* name, std::initializer_list<const Tensor*> inpu
 // ---- linear ---------------------------------------------------------------------------------------------------------------------------
 
 struct LinearBackward : public Node {
-  SavedVariable x, w, z;
+  Kept x, w, z;
   int64_t act = 0;
   at::DimVector x_shape;
   std::string name() const override { return "MinigridLinearBackward"; }
@@ -180,7 +200,7 @@ struct LinearBackward : public Node {
     if (!grads[0].defined()) return out;
     refuse_tracing("the gradient of linear");
     refuse_tangents("the gradient of linear", {&grads[0]});
-    const Tensor x0 = x.unpack(), w0 = w.unpack(), z0 = act ? z.unpack(shared_from_this()) : Tensor();
+    const Tensor x0 = x.get("x"), w0 = w.get("weight"), z0 = act ? z.get_contiguous("what the activation's slope is told from", shared_from_this()) : Tensor();
     const bool want_x = task_should_compute_output(0), want_w = task_should_compute_output(1), want_b = task_should_compute_output(2);
     if (task_should_compute_output(3)) out[3] = grads[0];
     {
@@ -267,12 +287,12 @@ Tensor linear(const Tensor& x, const Tensor& w, const MaybeTensor& bias, int64_t
                          ptr(rm), rm.defined() ? row_stride(rm) : 0, ptr(y), n, ptr(z), ws.p(), ws.bytes));
   }
   if (node) {
-    node->x = keep(x, xm);
-    node->w = keep(w, wm);
+    node->x.put(x, xm);
+    node->w.put(w, wm);
     node->act = act;
     node->x_shape = at::DimVector(x.sizes());
     torch::autograd::set_history(y, node);
-    if (act) node->z = from_y ? SavedVariable(y, true) : SavedVariable(z, false);
+    if (act) node->z.put(from_y ? y : z, from_y);
   }
   return y;
 }
@@ -298,7 +318,7 @@ void check_logits(const Tensor& l) {
 // ---- policy loss ----------------------------------------------------------------------------------------------------------------------
 
 struct PolicyLossBackward : public Node {
-  SavedVariable logits, action, mask, save;
+  Kept logits, action, mask, save;
   Tensor ready;                // the gradient for the factor 1, until a backward pass hands it out
   bool masked = false;
   uint64_t capture = 0;        // that the forward pass belongs to
@@ -319,7 +339,7 @@ struct PolicyLossBackward : public Node {
     if (!grads[0].defined() || !task_should_compute_output(0)) return out;
     refuse_tracing("the gradient of policy_loss");
     refuse_tangents("the gradient of policy_loss", {&grads[0]});
-    const Tensor l0 = logits.unpack(), a0 = action.unpack(), m0 = masked ? mask.unpack() : Tensor(), s0 = save.unpack();
+    const Tensor l0 = logits.get("logits"), a0 = action.get_contiguous("action"), m0 = masked ? mask.get_contiguous("mask") : Tensor(), s0 = save.get_contiguous("the rows' statistics");
     {
       at::AutoDispatchBelowADInplaceOrView below;
       const Tensor l = matrix(l0, shape.back());
@@ -374,11 +394,11 @@ std::pair<Tensor, Tensor> policy_loss(const Tensor& logits, const Tensor& action
     stats = out.narrow(0, 1, 5);
   }
   if (node) {
-    node->logits = keep(logits, l);
-    node->action = keep(action, a);
+    node->logits.put(logits, l);
+    node->action.put(action, a);
     node->masked = m.defined();
-    if (m.defined()) node->mask = keep(*mask, m);
-    node->save = SavedVariable(save, false);
+    if (m.defined()) node->mask.put(*mask, m);
+    node->save.put(save);
     node->ready = grad;
     node->capture = capture_on(dev);
     node->ent = ent;

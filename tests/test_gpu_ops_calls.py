@@ -283,3 +283,46 @@ def test_rollout_behind_fused_steps():
     traj = envs.rollout(3, policy=toy_policy)
     assert torch.equal(traj.image[0], image) and torch.equal(traj.done, done)
     envs.close()
+
+
+def kept_calls():
+    """operators whose backward pass reads every kind of tensor that they keep"""
+    x, w, b, r, dy = linear_inputs(50, 24, 40, torch.bfloat16, False, True, True, False, 5)
+    l, a, old, adv, ref, mask = loss_inputs(41, 7, torch.bfloat16, 3)
+    l2, a2, old2, adv2, ref2, mask2 = loss_inputs(41, 130, torch.float32, 3)
+    leaf = lambda t: t.detach().clone().requires_grad_(True)
+    x, w, b, l, l2 = leaf(x), leaf(w), leaf(b), leaf(l), leaf(l2)
+    two = torch.full((), 2.0, device="cuda")
+    return {"silu": (lambda: mg().linear(x, w, b, activation="silu"), [x, w, b], dy), "relu": (lambda: mg().linear(x, w, b, activation="relu"), [x, w, b], dy),
+            "leading": (lambda: mg().linear(x.view(5, 10, 24), w, b, activation="tanh"), [x, w, b], dy.view(5, 10, 40)),
+            "loss": (lambda: mg().policy_loss(l, a, old, adv, mask=mask, ref_log_prob=ref, kl_coef=0.1)[0], [l], two),
+            "long loss": (lambda: mg().policy_loss(l2, a2.int(), old2, adv2, mask=mask2, entropy_coef=0.1)[0], [l2], two)}
+
+
+@pytest.mark.parametrize("name", ["silu", "relu", "leading", "loss", "long loss"])
+def test_saved_tensor_hooks_that_give_back_other_strides(name):
+    """the same numbers at other addresses: columns first, or every second element of a row"""
+    f, leaves, dy = kept_calls()[name]
+    want = torch.autograd.grad(f(), leaves, dy)
+    for other in (lambda t: t.transpose(0, -1).contiguous().transpose(0, -1) if t.dim() else t.clone(), lambda t: torch.stack([t, t], -1)[..., 0]):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, other):
+            y = f()
+        for p, q in zip(torch.autograd.grad(y, leaves, dy), want):
+            assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("name", ["silu", "relu", "leading", "loss", "long loss"])
+def test_saved_tensor_hooks_that_give_back_something_else_are_refused(name):
+    """another type, shape or device, one kept tensor at a time"""
+    f, leaves, dy = kept_calls()[name]
+    kept = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: kept.append(t), lambda i: None):
+        f()
+    assert len(kept) >= 3
+    for at in range(len(kept)):
+        for other in (lambda t: t.to(torch.float16 if t.dtype != torch.float16 else torch.bfloat16), lambda t: t[:-1], lambda t: t.cpu()):
+            count = iter(range(len(kept)))
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: (next(count), t), lambda p: other(p[1]) if p[0] == at else p[1]):
+                y = f()
+            with pytest.raises(RuntimeError, match="saved-tensor hook"):
+                torch.autograd.grad(y, leaves, dy)
