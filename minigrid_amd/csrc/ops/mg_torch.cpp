@@ -90,8 +90,12 @@ struct Scratch {
 };
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
+// (a real tensor may carry a minus sign that is still to be applied: its memory does not hold its values)
+Tensor values(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+
 // t as (rows, cols) with contiguous columns and rows that do not overlap: the tensor's own memory where its strides allow it, else a copy
-Tensor matrix(const Tensor& t, int64_t cols) {
+Tensor matrix(const Tensor& signed_t, int64_t cols) {
+  const Tensor t = values(signed_t);
   Tensor m = t.dim() == 2 ? t : t.reshape({t.numel() / cols, cols});
   if ((cols > 1 && m.stride(1) != 1) || (m.size(0) > 1 && m.stride(0) < cols)) m = m.contiguous();
   return m;
@@ -119,7 +123,7 @@ struct Kept {
                 at::IntArrayRef(sizes), " on ", dev, ", and a saved-tensor hook gave back another type, shape or device");
     return t;
   }
-  Tensor get_contiguous(const char* name, std::shared_ptr<Node> owner = nullptr) const { return get(name, std::move(owner)).contiguous(); }
+  Tensor get_contiguous(const char* name, std::shared_ptr<Node> owner = nullptr) const { return values(get(name, std::move(owner))).contiguous(); }
   void reset_data() { saved.reset_data(); }
 };
 
@@ -275,7 +279,7 @@ Tensor linear(const Tensor& x, const Tensor& w, const MaybeTensor& bias, int64_t
     at::AutoDispatchBelowADInplaceOrView below;
     xm = matrix(x, k);
     wm = matrix(w, k);
-    const Tensor bc = b.defined() ? b.contiguous() : b, rm = r.defined() ? matrix(r, n) : r;
+    const Tensor bc = b.defined() ? values(b).contiguous() : b, rm = r.defined() ? matrix(r, n) : r;
     const int64_t rows = xm.size(0);
     const int dt = dtype_of(type);
     y = make(shape, type, dev);
@@ -307,7 +311,7 @@ Tensor per_row(const char* name, const Tensor& t, at::IntArrayRef shape, at::Dev
   if (!fine) refuse(name, " must be ", shape, " of ", at::ArrayRef<at::ScalarType>(types), ", got ", t.sizes(), " of ", t.scalar_type());
   if (t.requires_grad() && at::GradMode::is_enabled()) refuse(name, " is a constant of this operator and gets no gradient: pass ", name, ".detach()");
   at::AutoDispatchBelowADInplaceOrView below;
-  return t.contiguous();
+  return values(t).contiguous();
 }
 
 void check_logits(const Tensor& l) {
@@ -342,7 +346,7 @@ struct PolicyLossBackward : public Node {
     const Tensor l0 = logits.get("logits"), a0 = action.get_contiguous("action"), m0 = masked ? mask.get_contiguous("mask") : Tensor(), s0 = save.get_contiguous("the rows' statistics");
     {
       at::AutoDispatchBelowADInplaceOrView below;
-      const Tensor l = matrix(l0, shape.back());
+      const Tensor l = matrix(l0, shape.back()), factor = values(grads[0]).contiguous();
       const at::Device dev = l.device();
       // (a pass that is captured behind a forward pass outside of its own capture may be replayed several times behind one forward pass, and would then find
       // what it handed out before, as the caller left it)
@@ -350,7 +354,7 @@ struct PolicyLossBackward : public Node {
       out[0] = made ? std::move(ready) : make(shape, l.scalar_type(), dev);
       ready = Tensor();
       check((made ? L.mg_op_policy_loss_rescale : L.mg_op_policy_loss_backward)(dev.index(), stream_of(dev), dtype_of(l.scalar_type()), l.size(0), l.size(1), ptr(l), row_stride(l), ptr(a0),
-                                         dtype_of(a0.scalar_type()), (const uint8_t*)ptr(m0), ent, ptr(s0), (const float*)ptr(grads[0]), ptr(out[0])));
+                                         dtype_of(a0.scalar_type()), (const uint8_t*)ptr(m0), ent, ptr(s0), (const float*)ptr(factor), ptr(out[0])));
     }
     return no_second("policy_loss", std::move(out), {&grads[0], &l0});
   }
@@ -466,9 +470,10 @@ std::tuple<Tensor, Tensor, Tensor> advantages(const Tensor& reward, const Tensor
   a.steps = steps;
   a.envs = envs;
   auto strides = [](int64_t (&s)[2], const Tensor& t) { s[0] = t.stride(0); s[1] = t.stride(1); };
-  a.reward = ptr(reward); strides(a.s_reward, reward);
-  a.value = ptr(value); strides(a.s_value, value);
-  if (final_value) { a.final_value = ptr(*final_value); strides(a.s_final, *final_value); }
+  const Tensor r = values(reward), v = values(value), f = final_value ? values(*final_value) : Tensor();
+  a.reward = ptr(r); strides(a.s_reward, r);
+  a.value = ptr(v); strides(a.s_value, v);
+  if (f.defined()) { a.final_value = ptr(f); strides(a.s_final, f); }
   a.terminated = (const uint8_t*)ptr(terminated); strides(a.s_term, terminated);
   a.truncated = (const uint8_t*)ptr(truncated); strides(a.s_trunc, truncated);
   a.last_value = ptr(last);

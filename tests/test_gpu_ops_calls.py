@@ -326,3 +326,38 @@ def test_saved_tensor_hooks_that_give_back_something_else_are_refused(name):
                 y = f()
             with pytest.raises(RuntimeError, match="saved-tensor hook"):
                 torch.autograd.grad(y, leaves, dy)
+
+
+def test_lazily_negated_tensors():
+    """a real tensor whose minus sign is still to be applied (the imaginary part of a conjugated tensor is one): the same numbers as from its values"""
+    neg, val = torch._neg_view, lambda t: torch._neg_view(t).resolve_neg()
+    c = torch.complex(*(torch.randn((20, 8), generator=gen(i), device="cuda") for i in range(2)))
+    assert c.conj().imag.is_neg() and neg(c.real).is_neg()
+    x, w, b, r, dy = linear_inputs(50, 24, 40, torch.float32, False, True, True, False, 5)
+    leaves = lambda f: [f(t).detach().requires_grad_(True) for t in (x, w, b, r)]
+    run = lambda l, g: torch.autograd.grad(mg().linear(l[0], l[1], l[2], activation="silu", residual=l[3]), l, g)
+    lazy, plain = leaves(neg), leaves(val)
+    assert lazy[0].is_neg() and not plain[0].is_neg()
+    assert torch.equal(mg().linear(*lazy[:3], residual=lazy[3]), mg().linear(*plain[:3], residual=plain[3]))
+    for p, q in zip(run(lazy, neg(dy)), run(plain, val(dy))):
+        assert torch.equal(p, q)
+    for vocab in (7, 100):
+        l, a, old, adv, ref, mask = loss_inputs(40, vocab, torch.float32, 3)
+        out = []
+        for f in (neg, val):
+            X = f(l).detach().requires_grad_(True)
+            loss, stats = mg().policy_loss(X, a, f(old), f(adv), mask=mask, ref_log_prob=f(ref), kl_coef=0.1)
+            d, = torch.autograd.grad(loss, X, f(torch.full((), 0.5, device="cuda")))
+            act, lp = mg().sample_actions(f(l), f(-torch.rand(40, generator=gen(1), device="cuda")))
+            out.append((loss, stats, d, act, lp))
+        assert all(torch.equal(p, q) for p, q in zip(*out)), vocab
+    t = torch.zeros((20, 8), dtype=torch.bool, device="cuda")
+    reward, value = c.conj().imag, neg(c.real)
+    last = neg(torch.randn(8, generator=gen(3), device="cuda"))
+    for p, q in zip(mg().advantages(reward, value, last, t, t), mg().advantages(reward.resolve_neg(), value.resolve_neg(), last.resolve_neg(), t, t)):
+        assert torch.equal(p, q)
+    cut = t.clone()
+    cut[5] = True
+    for p, q in zip(mg().advantages(reward, value, last, t, cut, autoreset_mode="same_step", final_value=value),
+                    mg().advantages(reward.resolve_neg(), value.resolve_neg(), last.resolve_neg(), t, cut, autoreset_mode="same_step", final_value=value.resolve_neg())):
+        assert torch.equal(p, q)
