@@ -27,12 +27,12 @@ MG_API const char* mg_ops_last_error(void);
 
 /* ---- a layer of a policy network: y = act(x wT + b) + r ----
  * x (rows, k) of `dtype` or bytes (x_dtype = MG_DT_U8: an observation as the environments write it), w (n, k), b (n) or NULL, r (rows, n) or NULL,
- * y (rows, n), all of `dtype` (f32, bf16, f16).  z (rows, n, contiguous) or NULL: the values in front of the activation, for the backward pass.  Sums
- * are held in 32 bits.  act = gelu is x Phi(x) with the normal distribution function itself. */
+ * y (rows, n), all of `dtype` (f32, bf16, f16).  z (rows, n, contiguous; `dtype`, for tanh f32) or NULL: the values in front of the activation, for the
+ * backward pass.  Sums are held in 32 bits.  act = gelu is x Phi(x) with the normal distribution function itself. */
 MG_API int mg_op_linear_workspace(int64_t rows, int64_t k, int64_t n, int dtype, int64_t* forward, int64_t* backward_input, int64_t* backward_weight);
 MG_API int mg_op_linear(int device, void* stream, int dtype, int x_dtype, int act, int64_t rows, int64_t k, int64_t n, const void* x, int64_t ldx,
                         const void* w, int64_t ldw, const void* b, const void* r, int64_t ldr, void* y, int64_t ldy, void* z, void* ws, int64_t ws_bytes);
-/* dz = dy * act'(z) (rows, n, contiguous; NULL allowed for act = none) and db = the column sums of dz (n, `dtype`; NULL = not wanted).
+/* dz = dy * act'(z), z as the forward pass has left it (dz: rows, n, contiguous; NULL allowed for act = none) and db = the column sums of dz (n, `dtype`; NULL = not wanted).
  * ws: mg_op_linear_dz_workspace bytes (needed for db only). */
 MG_API int mg_op_linear_dz_workspace(int64_t rows, int64_t n, int64_t* bytes);
 MG_API int mg_op_linear_dz(int device, void* stream, int dtype, int act, int64_t rows, int64_t n, const void* dy, int64_t lddy, const void* z, void* dz,

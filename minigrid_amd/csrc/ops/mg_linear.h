@@ -40,7 +40,7 @@ struct Epilogue {
   const void* b;   // (n) or null
   const void* r;   // (rows, n) or null
   void* c;         // result of T, row stride ldc
-  void* z;         // values in front of the activation (contiguous), or null
+  void* z;         // values in front of the activation (contiguous, of KeptOf<T, act>), or null
   float* part;     // split sums: f32 (splits, rows, n), contiguous; null = store the result
   int64_t ldr, ldc;
   int32_t act;
@@ -48,6 +48,12 @@ struct Epilogue {
 };
 
 // ---- activations ----
+// What a backward pass keeps of z.  For most activations z in the operands' type: the slope at a rounded z is off by less than dz's own rounding (by a third of it for
+// gelu and silu at z of 1).  tanh's slope falls as e^{-2 |z|}, so at a rounded z it would be off by 2 |z| half steps of itself: z stays in 32 bits.  (dx and
+// dw of 2 049 x 300 x 136 bf16 are off by 2.55e-3 of their norm with a rounded z, 2.33e-3 without, by 1.66e-3 where they alone are rounded; the forward and backward
+// pass of 65 536 x 512 x 512 take 238 and 253 us.)
+template <class T, int ACT> using KeptOf = std::conditional_t<ACT == MG_ACTIVATION_TANH, float, T>;
+
 // exp2 with a result of 0 far below the smallest number: v_exp_f32, one ulp
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float rcp_fast(float x) { return __builtin_amdgcn_rcpf(x); }
@@ -276,7 +282,10 @@ template <class T> __device__ __forceinline__ float activate_any(int act, float 
 template <class T>
 __device__ __forceinline__ void finish(const Epilogue& e, int64_t i, int64_t j, int64_t n, float v) {
   if (e.b) v += (float)((const T*)e.b)[j];
-  if (e.z) ((T*)e.z)[i * n + j] = (T)v;
+  if (e.z) {
+    if (e.act == MG_ACTIVATION_TANH) ((float*)e.z)[i * n + j] = v;
+    else ((T*)e.z)[i * n + j] = (T)v;
+  }
   v = activate_any<T>(e.act, v);
   if (e.r) v += (float)((const T*)e.r)[i * e.ldr + j];
   ((T*)e.c)[i * e.ldc + j] = (T)v;
@@ -371,7 +380,7 @@ __device__ __forceinline__ void store_tile(const Epilogue& ep, f32x16 (&acc)[MI]
         }
 #pragma unroll
         for (int e = 0; e < W; e++) v[u][e] += bias[e];
-        if (ep.z) store_some<T, W>((T*)ep.z + i * n + j, v[u], skip, count);
+        if (ep.z) store_some<KeptOf<T, ACT>, W>((KeptOf<T, ACT>*)ep.z + i * n + j, v[u], skip, count);
 #pragma unroll
         for (int e = 0; e < W; e++) v[u][e] = activate(ACT, v[u][e]);
         if (residual)
@@ -452,7 +461,9 @@ __device__ __forceinline__ void store_wave(const Epilogue& ep, f32x16 (&acc)[MI]
     }
     return;
   }
-  const VIEW c(ep.c, i0, j0, ep.ldc, SZ), z(ep.z, i0, j0, n, SZ), r(ep.r, i0, j0, ep.ldr, SZ);
+  typedef KeptOf<T, ACT> Z;
+  typedef Z Z8 __attribute__((ext_vector_type(8)));
+  const VIEW c(ep.c, i0, j0, ep.ldc, SZ), z(ep.z, i0, j0, n, sizeof(Z)), r(ep.r, i0, j0, ep.ldr, SZ);
   float bias[8] = {};
   if (ep.b) {
     V8 t;
@@ -460,7 +471,7 @@ __device__ __forceinline__ void store_wave(const Epilogue& ep, f32x16 (&acc)[MI]
 #pragma unroll
     for (int e = 0; e < 8; e++) bias[e] = (float)t[e];
   }
-  const uint32_t oc = r0 * c.row + col * SZ, oz = r0 * z.row + col * SZ;
+  const uint32_t oc = r0 * c.row + col * SZ, oz = r0 * z.row + col * sizeof(Z);
   constexpr int W = SZ / 2;                                      // 16-byte words of eight elements
   // (as many rows as registers hold: all of them, of 32-bit elements a half)
   constexpr int AHEAD = SZ == 2 ? H * P : P;
@@ -472,11 +483,11 @@ __device__ __forceinline__ void store_wave(const Epilogue& ep, f32x16 (&acc)[MI]
       for (int w = 0; w < W; w++) res[p][w] = r.get(r0 * r.row + col * SZ + w * 16, (first + p) * RPP * r.row);       // (rows and columns that are not its own lie inside too)
   };
   if constexpr (RES) residuals(0);
-  auto put8 = [&](const VIEW& v, bool own, uint32_t lane, uint32_t at, const V8& t) __attribute__((always_inline)) {
-    u32x4 d[W];
+  auto put8 = [&](const VIEW& v, bool own, uint32_t lane, uint32_t at, const auto& t) __attribute__((always_inline)) {
+    u32x4 d[sizeof t / 16];
     __builtin_memcpy(d, &t, sizeof d);
 #pragma unroll
-    for (int w = 0; w < W; w++) v.put(own, lane + w * 16, at, d[w]);
+    for (int w = 0; w < (int)(sizeof t / 16); w++) v.put(own, lane + w * 16, at, d[w]);
   };
   auto finish_row = [&](int h, int p, const u32x4 (&residual)[W]) __attribute__((always_inline)) {
     const int row = p * RPP + r0;
@@ -489,9 +500,10 @@ __device__ __forceinline__ void store_wave(const Epilogue& ep, f32x16 (&acc)[MI]
 #pragma unroll
     for (int e = 0; e < 8; e++) v[e] += bias[e];
     if (ep.z) {
+      Z8 kept;
 #pragma unroll
-      for (int e = 0; e < 8; e++) t[e] = (T)v[e];
-      put8(z, own, oz, step * z.row, t);
+      for (int e = 0; e < 8; e++) kept[e] = (Z)v[e];
+      put8(z, own, oz, step * z.row, kept);
     }
 #pragma unroll
     for (int e = 0; e < 8; e++) {

@@ -95,7 +95,7 @@ def linear(x, weight, bias=None, *, activation: Optional[str] = None, residual=N
     "gelu" (x Phi(x) with the normal distribution function itself) or "silu".  Sums are held in 32 bits and the result is rounded once.
 
     Differentiable in x (unless bytes), weight, bias and residual, once.  For the backward pass of an activation the values in front of it are kept
-    in weight's dtype (relu without a residual: the result itself, which must then not be changed in place), and their gradient is rounded to it before the two products that use it (the matrix instructions take such operands);
+    in weight's dtype (tanh: in float32, since its slope would lose most by that; relu without a residual: the result itself, which must then not be changed in place), and their gradient is rounded to it before the two products that use it (the matrix instructions take such operands);
     bias's gradient is summed before that rounding.  All sums run in a fixed order."""
     if activation not in _ACTIVATIONS:
         raise ValueError(f"activation must be one of {[a for a in _ACTIVATIONS if a]} or None")

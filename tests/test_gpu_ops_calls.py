@@ -8,7 +8,7 @@ import pytest
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
-from test_gpu_ops import DT, U, advantages64, check_loss, gen, linear_inputs, loss_inputs, mg, within
+from test_gpu_ops import DT, EL, U, advantages64, check_loss, gen, half, linear_inputs, loss_inputs, mg, run_linear, tiny, within
 
 
 @pytest.mark.parametrize("dt", ["bf16", "f32"])
@@ -361,3 +361,20 @@ def test_lazily_negated_tensors():
     for p, q in zip(mg().advantages(reward, value, last, t, cut, autoreset_mode="same_step", final_value=value),
                     mg().advantages(reward.resolve_neg(), value.resolve_neg(), last.resolve_neg(), t, cut, autoreset_mode="same_step", final_value=value.resolve_neg())):
         assert torch.equal(p, q)
+
+
+# few rows, guarded tiles, whole ones, the split and joined, the largest at aligned rows and at odd ones
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("rows,k,n,res", [(1, 147, 64, False), (8, 30, 33, True), (9, 30, 8, False), (40, 4096, 130, True), (200, 75, 96, False), (300, 513, 257, True), (2049, 300, 136, False),
+                                          (4104, 1032, 2056, True), (4103, 1031, 2055, False)])
+def test_linear_slope_of_tanh(dt, rows, k, n, res):
+    """tanh's slope at a rounded z would be off by 2 |z| half steps of it: what is kept for it is not rounded, so that bias's gradient, which is summed before anything is
+    rounded, is off by its own rounding, by that of 32-bit sums, and by EL for the slope"""
+    x, w, b, r, dy = linear_inputs(rows, k, n, DT[dt], False, True, res, False, 3)
+    w = (w.float() * 2).to(DT[dt])                                   # z as large as 2 and more
+    _, _, _, db = run_linear(x, w, b, r, dy, "tanh")
+    z, S = x.double() @ w.double().t() + b.double(), x.double().abs() @ w.double().abs().t() + b.double().abs()
+    dz = dy.double() * (1 - torch.tanh(z) ** 2)
+    es = dy.double().abs() * 0.8 * (k + 4) * U * S + EL * dz.abs()   # (no second derivative is above 0.8)
+    want = dz.sum(0)
+    within(db, want, es.sum(0) * 1.01 + (rows + 4) * U * (dz.abs() + es).sum(0) + half(DT[dt]) * (1.01 * want.abs() + es.sum(0)) + tiny(DT[dt]), "db")
