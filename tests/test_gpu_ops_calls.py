@@ -378,3 +378,67 @@ def test_linear_slope_of_tanh(dt, rows, k, n, res):
     es = dy.double().abs() * 0.8 * (k + 4) * U * S + EL * dz.abs()   # (no second derivative is above 0.8)
     want = dz.sum(0)
     within(db, want, es.sum(0) * 1.01 + (rows + 4) * U * (dz.abs() + es).sum(0) + half(DT[dt]) * (1.01 * want.abs() + es.sum(0)) + tiny(DT[dt]), "db")
+
+
+# rows of every class that a workgroup's registers hold, at its first and last sizes: 16, 32, 80 and 160 KB
+@pytest.mark.parametrize("dt,vocab", [(t, n) for t, sizes in (("f32", (4096, 4097, 4099, 4100, 8192, 8193, 8196, 20480, 20483, 20484, 20485, 40959, 40960)),
+                                                              ("bf16", (8192, 8193, 8199, 8200, 16384, 16391, 16392, 40960, 40967, 40968, 40969, 81919, 81920)),
+                                                              ("f16", (8193, 16385, 40969, 81920))) for n in sizes])
+def test_policy_loss_held_rows(dt, vocab):
+    for gap, padded in ((0, 0.3), (1, 0.0), (3, 0.3)):
+        check_loss(*loss_inputs(11, vocab, DT[dt], vocab + gap, gap=gap, padded=padded, ref=gap != 1), scale=8.0 if dt == "f16" else 1.0)
+
+
+@pytest.mark.parametrize("dt,vocab", [("f32", 70), ("f32", 5001), ("f32", 20487), ("bf16", 131), ("bf16", 9001), ("bf16", 41003)])
+def test_policy_loss_held_rows_several_to_a_workgroup(dt, vocab):
+    check_loss(*loss_inputs(8195, vocab, DT[dt], 3, gap=1, padded=0.3))
+
+
+def recurrence64(r, v, last, term, trunc, gamma, lam, mode, done=None, final=None):
+    """(advantages64 with the environments side by side)"""
+    T, N = v.shape
+    r, v, last = r.double(), v.double(), last.double()
+    term, trunc = term != 0, trunc != 0
+    ends, zero = term | trunc, torch.zeros(N, dtype=torch.float64, device="cuda")
+    resets = torch.zeros_like(ends)
+    if mode == "next_step":
+        resets[1:] = ends[:-1]
+        resets[0] = done != 0 if done is not None else False
+    adv, run = torch.zeros_like(v), zero
+    for t in reversed(range(T)):
+        worth = v[t + 1] if t + 1 < T else last
+        if mode == "same_step":
+            worth = torch.where(trunc[t], final[t].double() if final is not None else zero, worth)
+        worth = torch.where(term[t], zero, worth)
+        run = r[t] + gamma * worth - v[t] + torch.where(ends[t], zero, gamma * lam * run)
+        run = torch.where(resets[t], zero, run)
+        adv[t] = run
+    return adv, adv + v, ~resets
+
+
+@pytest.mark.parametrize("envs", [32768, 32805, 40000])
+@pytest.mark.parametrize("steps", [16, 17, 33, 128, 129, 300])
+@pytest.mark.parametrize("mode", ["next_step", "same_step"])
+def test_advantages_of_many_environments(envs, steps, mode):
+    """64 environments a workgroup, one stretch and several, one block of stretches and several"""
+    g = gen(steps + envs)
+    apart = steps % 2 == 0
+    rec = torch.zeros((steps, envs, 16), dtype=torch.uint8, device="cuda")
+    r = rec.view(torch.float64)[:, :, 0]
+    r.copy_(torch.randn((steps, envs), generator=g, device="cuda"))
+    ends = torch.rand((steps, envs), generator=g, device="cuda")
+    rec[:, :, 8], rec[:, :, 9] = ends < 0.02, (ends > 0.015) & (ends < 0.04)
+    term, trunc = rec[:, :, 8], rec[:, :, 9]
+    if apart:
+        r, term, trunc = r.float(), term.bool(), trunc.bool()
+    vt = [torch.float32, torch.bfloat16, torch.float16][(steps + envs) % 3]
+    f = lambda *s: torch.randn(s, generator=g, device="cuda").to(vt)
+    v, last = f(steps, envs), f(envs)
+    done = torch.rand(envs, generator=g, device="cuda") < 0.3 if mode == "next_step" else None
+    final = f(steps, envs) if mode == "same_step" and steps % 3 else None
+    args = (r, v, last, term, trunc)
+    wa, wr, wv = recurrence64(*args, 0.97, 0.9, mode, done, final)
+    adv, ret, valid = mg().advantages(*args, gamma=0.97, lam=0.9, autoreset_mode=mode, done=done, final_value=final)
+    assert torch.equal(valid, wv)
+    within(adv, wa, 1.01 * U * wa.abs() + 1e-12, "advantage")
+    within(ret, wr, 1.01 * U * wr.abs() + 1e-12, "return")
