@@ -7,26 +7,45 @@ namespace mgo {
 // The unchecked kernel needs a whole tile of every axis, and a tile of an operand that spans less than 2 GiB (one 32-bit offset per thread).
 static bool fits(int tile, int64_t ri, int64_t rj, int64_t depth, int bk) { return ri >= TILE_I[tile] && rj >= TILE_J[tile] && depth >= bk; }
 
-// The largest tile with which the CUs are busy, the summed axis split where the tiles of the result alone do not do that (in runs of at least four tiles).
-// A CU holds one workgroup of the 256-tile, two of 128, four of 64.  Where the 256-tiles would have to be split and the 128-tiles fill the CUs by themselves, those:
-// 3 297 x 1 483 x 2 096 66 us against 58, 6 000 x 3 003 x 1 001 86 against 72; at 256 tiles of 128 the split 256-tiles are ahead (1 024 x 4 096 x 4 096 58 against 66),
-// and along a long axis (4 096 x 32 768 x 2 048 467 against 770).
-static Plan plan_product(int64_t ri, int64_t rj, int64_t depth, int dtype) {
+// A tile and how the summed axis is split: as often as the CUs hold workgroups that the tiles of the result alone do not fill (in runs of at least four tiles).  A
+// CU holds one workgroup of the 256-tile, two of 128, four of 64.
+static Plan with_tile(int tile, int64_t ri, int64_t rj, int64_t deep) {
+  const int64_t slots = tile == TILE_256 ? 256 : tile == TILE_64 ? 1024 : 512, tiles = ceil_div(ri, TILE_I[tile]) * ceil_div(rj, TILE_J[tile]);
   Plan p;
-  const int bk = 128 / dtype_bytes(dtype);
-  const int64_t deep = ceil_div(depth, bk);
-  auto tiles = [&](int t) { return ceil_div(ri, TILE_I[t]) * ceil_div(rj, TILE_J[t]); };
-  int64_t slots;
-  if (fits(TILE_256, ri, rj, depth, bk) && tiles(TILE_256) * deep >= 256 * 8 && (tiles(TILE_256) >= 200 || tiles(TILE_128) < 300 || deep > 64)) { p.tile = TILE_256; slots = 256; }
-  else if (fits(TILE_128, ri, rj, depth, bk) && tiles(TILE_128) * deep >= 256 * 4) { p.tile = TILE_128; slots = 512; }
-  else if (fits(TILE_64, ri, rj, depth, bk)) { p.tile = TILE_64; slots = 1024; }
-  else { p.tile = ri <= 32 ? TILE_GUARDED_32_128 : rj <= 32 ? TILE_GUARDED_128_32 : TILE_GUARDED_128_128; slots = 512; }
-  int64_t splits = std::max<int64_t>(1, slots / tiles(p.tile));
-  splits = std::max<int64_t>(1, std::min(splits, deep / 4));
+  p.tile = tile;
+  const int64_t splits = std::max<int64_t>(1, std::min(slots / tiles, deep / 4));
   p.per = (int)ceil_div(deep, splits);
   p.splits = p.per ? (int)ceil_div(deep, p.per) : 1;
   p.part_bytes = p.splits > 1 ? (int64_t)p.splits * ri * rj * 4 : 0;
   return p;
+}
+
+// About how many us the product takes: rounds of one workgroup a CU (two of a CU share its matrix units), each as long as its piece of the summed axis, and the splits'
+// sums, which are written and read at 4 TB/s.  ns per summed element and workgroup, measured with the CUs full: 4 096 x 4 096 x 8 192 bf16 in 199 us with 256-tiles, 317
+// with 128; 4 096 x 4 096 x 2 048 f32 in 510 and 545.
+static double about_us(const Plan& p, int64_t ri, int64_t rj, int64_t depth, int dtype) {
+  const bool f32 = dtype == MG_DT_F32, large = p.tile == TILE_256;
+  const double ns = large ? (f32 ? 250.0 : 24.6) : (f32 ? 66.0 : 9.7);
+  const int64_t rounds = ceil_div(ceil_div(ri, TILE_I[p.tile]) * ceil_div(rj, TILE_J[p.tile]) * p.splits, 256);
+  return rounds * (double)std::min<int64_t>(depth, (int64_t)p.per * (128 / dtype_bytes(dtype))) * ns * 1e-3 + 2.0 * p.part_bytes * 0.25e-6;
+}
+
+// 256-tiles or 128?  For 16-bit operands the large ones multiply faster, but leave more CUs idle in the last round, and need more splits.  The estimates decide, with 5 % for
+// the large ones.  Over 257 products (21 shapes of 256 x 512 to 65 536 x 512, 512 to 65 536 summed, both types, forward and dw) what they choose is 0.4 % slower than the
+// better of the two in the mean, at most 15 %: 3 328 x 3 328 x 2 048 bf16 256 46 us (128: 68), 3 297 x 1 483 x 2 048 bf16 128 41 (256: 48), 2 304 x 2 304 x 4 096 bf16 256 62
+// (128: 76), 6 000 x 3 003 x 1 001 f32 128 345 (256: 513).
+static Plan plan_product(int64_t ri, int64_t rj, int64_t depth, int dtype) {
+  const int bk = 128 / dtype_bytes(dtype);
+  const int64_t deep = ceil_div(depth, bk);
+  auto work = [&](int t) { return ceil_div(ri, TILE_I[t]) * ceil_div(rj, TILE_J[t]) * deep; };
+  if (fits(TILE_128, ri, rj, depth, bk) && work(TILE_128) >= 256 * 4) {
+    const Plan p = with_tile(TILE_128, ri, rj, deep);
+    if (!fits(TILE_256, ri, rj, depth, bk) || work(TILE_256) < 256 * 8) return p;
+    const Plan large = with_tile(TILE_256, ri, rj, deep);
+    return about_us(large, ri, rj, depth, dtype) <= 1.05 * about_us(p, ri, rj, depth, dtype) ? large : p;
+  }
+  if (fits(TILE_64, ri, rj, depth, bk)) return with_tile(TILE_64, ri, rj, deep);
+  return with_tile(ri <= 32 ? TILE_GUARDED_32_128 : rj <= 32 ? TILE_GUARDED_128_32 : TILE_GUARDED_128_128, ri, rj, deep);
 }
 
 template <class F> static int by_type(int dtype, F f) {
