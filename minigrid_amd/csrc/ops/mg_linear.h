@@ -59,7 +59,9 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 __device__ __forceinline__ float rcp_fast(float x) { return __builtin_amdgcn_rcpf(x); }
 
 // The normal distribution function at -|x|: e^{-x^2/2} q(t), t = 1 / (1 + 0.3 |x|).  q is 0.5 erfcx(|x| / sqrt 2) as a polynomial of degree 8 without a
-// constant term, fitted here for the least largest RELATIVE error on |x| <= 13.5 (1.3e-7; 2.9e-7 evaluated in 32 bits); beyond, e^{-x^2/2} is 0 in f32.
+// constant term, fitted here for the least largest RELATIVE error on |x| <= 13.5 (1.3e-7; 2.9e-7 evaluated in 32 bits); beyond, e^{-x^2/2} is 0 in f32.  The exponential
+// adds what rounding its argument to 32 bits makes: gelu(-x) is off by 7e-7 of itself up to 3, 2e-6 at 6, 8e-6 at 13, where it is 1e-37.  (tanh's slope, from
+// e^{-2 |z|}: 6e-7 up to 3, 1.1e-6 at 9, 4e-6 at 40; silu: 6e-7 at -9, 2e-6 at -40.)
 __device__ __forceinline__ float phi_tail(float a, float* density) {
   const float t = rcp_fast(__builtin_fmaf(0.3f, a, 1.0f));
   float q = 0.03593193367123604f;
@@ -270,15 +272,6 @@ __device__ __forceinline__ f32x16 mma(f32x4 a, f32x4 b, f32x16 c) {   // both op
 }
 
 // one element of the result; the sum comes in 32 bits and each result is rounded to T once
-template <class T> __device__ __forceinline__ float activate_any(int act, float z) {
-  switch (act) {
-    case MG_ACTIVATION_RELU: return activate(MG_ACTIVATION_RELU, z);
-    case MG_ACTIVATION_TANH: return activate(MG_ACTIVATION_TANH, z);
-    case MG_ACTIVATION_GELU: return activate(MG_ACTIVATION_GELU, z);
-    case MG_ACTIVATION_SILU: return activate(MG_ACTIVATION_SILU, z);
-    default: return z;
-  }
-}
 template <class T>
 __device__ __forceinline__ void finish(const Epilogue& e, int64_t i, int64_t j, int64_t n, float v) {
   if (e.b) v += (float)((const T*)e.b)[j];
@@ -286,7 +279,7 @@ __device__ __forceinline__ void finish(const Epilogue& e, int64_t i, int64_t j, 
     if (e.act == MG_ACTIVATION_TANH) ((float*)e.z)[i * n + j] = v;
     else ((T*)e.z)[i * n + j] = (T)v;
   }
-  v = activate_any<T>(e.act, v);
+  v = activate(e.act, v);
   if (e.r) v += (float)((const T*)e.r)[i * e.ldr + j];
   ((T*)e.c)[i * e.ldc + j] = (T)v;
 }

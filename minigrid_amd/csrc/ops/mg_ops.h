@@ -17,7 +17,6 @@ typedef __bf16 bf16;
 typedef _Float16 f16;
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 int fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));   // sets mg_ops_last_error() of this thread
 int launched(const char* what);                                                   // MG_OK, or what hipGetLastError says
@@ -39,8 +38,6 @@ struct DeviceGuard {
 
 inline int dtype_bytes(int d) { return d == MG_DT_F32 || d == MG_DT_I32 ? 4 : d == MG_DT_BF16 || d == MG_DT_F16 ? 2 : d == MG_DT_F64 || d == MG_DT_I64 ? 8 : d == MG_DT_U8 ? 1 : 0; }
 
-template <class T> __device__ __forceinline__ float to_f32(T v) { return (float)v; }
-
 // ---- wave reductions ----
 __device__ __forceinline__ double shfl_xor_f64(double v, int m) {
   int lo = __double2loint(v), hi = __double2hiint(v);
@@ -58,8 +55,7 @@ __device__ __forceinline__ float wave_max(float v) {
   return v;
 }
 
-constexpr float LOG2E_HI = 1.44269504f;            // log2(e) = HI + LO to about 48 bits
-constexpr float LOG2E_LO = 1.92596303e-8f;
+constexpr float LOG2E = 1.44269504f;
 constexpr double LN2 = 0.693147180559945309417232;
 
 }  // namespace mgo

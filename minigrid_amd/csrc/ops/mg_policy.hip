@@ -182,7 +182,7 @@ __device__ __forceinline__ void add_chunk(Sums& a, const float (&x)[N]) {
     for (int u = g; u < g + G; u++) {
       float d = x[u] - a.m;
       d = d < -200.0f ? -200.0f : d;                             // e^-200 is 0 in 32 bits, and 0 * -200 is 0 (keeps a NaN)
-      const float e = __builtin_amdgcn_exp2f(d * LOG2E_HI);
+      const float e = __builtin_amdgcn_exp2f(d * LOG2E);
       s += e;
       t = __builtin_fmaf(e, d, t);
     }
@@ -240,7 +240,7 @@ struct GradArgs {
 __device__ __forceinline__ float grad_of(float l, double lse, float entropy, float dlp, float ent, bool chosen) {
   float d = (float)((double)l - lse);
   d = d < -200.0f ? -200.0f : d;
-  const float p = __builtin_amdgcn_exp2f(d * LOG2E_HI);
+  const float p = __builtin_amdgcn_exp2f(d * LOG2E);
   return p * (ent * (d + entropy) - dlp) + (chosen ? dlp : 0.0f);
 }
 
@@ -277,11 +277,11 @@ __global__ void k_grad_small(GradArgs a) {
 struct GradRow {
   float hi, lo2, ent2, k, dlp;
   __device__ __forceinline__ GradRow(const Saved& s, float dlp_, float ent) : hi((float)s.lse), ent2(ent * (float)LN2), dlp(dlp_) {
-    lo2 = (float)(s.lse - (double)hi) * LOG2E_HI;
+    lo2 = (float)(s.lse - (double)hi) * LOG2E;
     k = __builtin_fmaf(ent, s.entropy, -dlp_);
   }
   __device__ __forceinline__ float operator()(float l) const {
-    const float y = __builtin_fmaf(l - hi, LOG2E_HI, -lo2);
+    const float y = __builtin_fmaf(l - hi, LOG2E, -lo2);
     return __builtin_amdgcn_exp2f(y) * __builtin_fmaf(ent2, fmaxf(y, -300.0f), k);           // (a NaN is in the first factor, and a closed column's is 0)
   }
   // the chunk of columns c..c + N
@@ -443,7 +443,7 @@ __global__ __launch_bounds__(NT, 4) void k_loss_held(LossArgs a, double* part, c
     for (int w = 1; w < W; w++) m = fmaxf(m, wm[w]);
     double s = 0.0, t = 0.0;
     auto add = [&](float x, float& e8, float& t8) __attribute__((always_inline)) {
-      const float z = (x - m) * LOG2E_HI, e = __builtin_amdgcn_exp2f(z);
+      const float z = (x - m) * LOG2E, e = __builtin_amdgcn_exp2f(z);
       e8 += e;
       t8 = __builtin_fmaf(e, fmaxf(z, -300.0f), t8);             // (2^-300 is 0 in 32 bits; a NaN is in e)
     };
