@@ -14,6 +14,8 @@
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>
 
+#include <unordered_set>
+
 #include "../../../include/minigrid_ops.h"
 
 namespace {
@@ -158,17 +160,28 @@ uint64_t capture_on(at::Device dev) {
   return status == hipStreamCaptureStatusNone ? 0 : id;
 }
 
-// A captured step must not meet an eager graph of the same leaves that is still alive: the leaves' gradient nodes belong to the stream that graph was recorded
-// on, the backward pass would wait on that stream from inside the capture, and torch ends the process there.  Said here, where it can still be said.
+// A captured step must not meet an eager graph of the same leaves that is still alive, or go on from one: the leaves' gradient nodes (or that graph's own) belong to the
+// stream that it was recorded on, the backward pass would wait on that stream from inside the capture, and torch ends the process there.  Said here, where it can
+// still be said, of everything that the inputs were made from.
 void refuse_capture_beside_eager(at::Device dev, std::initializer_list<const Tensor*> inputs) {
   if (!capture_on(dev)) return;
+  const auto here = c10::hip::getCurrentHIPStream(dev.index()).id();
+  std::vector<std::shared_ptr<Node>> todo;
+  std::unordered_set<Node*> seen;
   for (const Tensor* t : inputs) {
-    if (!t->defined() || !t->requires_grad() || t->grad_fn()) continue;
-    const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
-    if (!node) continue;
+    if (!t->defined() || !t->requires_grad()) continue;
+    // (a leaf's gradient node is looked at where there is one, not made)
+    if (auto node = t->grad_fn() ? t->grad_fn() : torch::autograd::impl::try_get_grad_accumulator(*t)) todo.push_back(std::move(node));
+  }
+  while (!todo.empty()) {
+    const auto node = std::move(todo.back());
+    todo.pop_back();
+    if (!seen.insert(node.get()).second) continue;
     const auto at = node->stream();
-    if (at && at->id() != c10::hip::getCurrentHIPStream(t->device().index()).id())
+    if (at && at->id() != here)
       refuse("a tensor that requires a gradient is still part of a graph recorded outside of this capture: drop that graph's results before capturing");
+    for (const auto& edge : node->next_edges())
+      if (edge.function) todo.push_back(edge.function);
   }
 }
 

@@ -442,3 +442,33 @@ def test_advantages_of_many_environments(envs, steps, mode):
     assert torch.equal(valid, wv)
     within(adv, wa, 1.01 * U * wa.abs() + 1e-12, "advantage")
     within(ret, wr, 1.01 * U * wr.abs() + 1e-12, "return")
+
+
+@pytest.mark.parametrize("op", ["linear", "policy_loss"])
+def test_capture_of_what_was_made_from_leaves_of_an_eager_graph_is_refused(op):
+    """(the backward pass would end the process.)  The leaves may be any number of operations away, and what the capture goes on from may itself be eager"""
+    x, a, old, adv, ref, mask = loss_inputs(40, 7, torch.float32, 3)
+    w = torch.randn((5, 7), generator=gen(1), device="cuda", requires_grad=True)
+    x = x.contiguous().requires_grad_(True)
+    call = {"linear": lambda x: mg().linear(x, (w * 1.0).detach(), activation="tanh").sum(), "policy_loss": lambda x: mg().policy_loss(x, a, old, adv)[0]}[op]
+    step = lambda: call((x * 2.0).tanh())
+    alive = x * 3.0                                                  # an eager graph of the leaf
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with pytest.raises(ValueError, match="outside of this capture"):
+        with torch.cuda.graph(g):
+            step()
+    del alive, g
+    before = x * 2.0                                                 # the capture goes on from an eager result
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with pytest.raises(ValueError, match="outside of this capture"):
+        with torch.cuda.graph(g):
+            call(before)
+    del before, g
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        d, = torch.autograd.grad(step(), [x])
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(d, torch.autograd.grad(step(), [x])[0])
