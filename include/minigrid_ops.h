@@ -9,6 +9,7 @@
  *   - stateless: no handle, no allocation, no synchronisation.  All pointers are device memory of `device`; work is enqueued on `stream` (a
  *     hipStream_t; NULL = the null stream).  A call may be captured into a graph.  Two calls that may run at once need two workspaces.
  *   - `ld*` are row strides in ELEMENTS; the columns of a row are contiguous.  Types are mg_dtype values.
+ *   - results overlap neither operands nor each other.
  *   - a workspace is scratch: its content before a call does not matter and after it means nothing; it has to be 256-byte aligned.
  */
 #ifndef MINIGRID_OPS_H
@@ -81,6 +82,7 @@ MG_API int mg_op_sample(int device, void* stream, int dtype, int64_t rows, int64
  * an episode ended in the step before the first; final_value or NULL (same_step only): the value of the observation a truncated step ended on.
  * next_step != 0 is the environments' default autoreset: the step behind an end only resets, counts for nothing (valid = 0, advantage 0), and its
  * observation is the one the episode ended on.  next_step = 0: the step behind an end is the first of the next episode.
+ * Where reward (f64), terminated and truncated are the first fields of 16-byte records at 16-byte addresses, as the environments write them, records are read whole.
  * advantage, ret (f32) and valid (u8): (steps, envs), contiguous. */
 typedef struct mg_advantages_args {
   int64_t steps, envs;

@@ -64,6 +64,6 @@ class Trajectory:
 
     def loss(self, logits, advantage, mask=None, *, index: Optional[torch.Tensor] = None, ref_log_prob=None, **kw):
         """`ops.policy_loss` of new logits for all transitions, or for those at `index` of the flattened (steps x envs) -- a minibatch; advantage, mask and
-        ref_log_prob are (steps, envs) either way."""
+        ref_log_prob are (steps, envs) either way.  In the next_step mode mask is `advantages`' valid: without it the rows that only reset count too."""
         pick = (lambda t: t) if index is None else (lambda t: None if t is None else t.reshape(-1)[index])
         return ops.policy_loss(logits, pick(self.action), pick(self.log_prob), pick(advantage), mask=pick(mask), ref_log_prob=pick(ref_log_prob), **kw)
