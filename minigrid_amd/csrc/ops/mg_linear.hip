@@ -31,7 +31,7 @@ static double about_us(const Plan& p, int64_t ri, int64_t rj, int64_t depth, int
 }
 
 // 256-tiles or 128?  For 16-bit operands the large ones multiply faster, but leave more CUs idle in the last round, and need more splits.  The estimates decide, with 5 % for
-// the large ones.  Over 257 products (21 shapes of 256 x 512 to 65 536 x 512, 512 to 65 536 summed, both types, forward and dw) what they choose is 0.4 % slower than the
+// the large ones.  Over 257 products (25 shapes of 256 x 512 to 65 536 x 512, 512 to 65 536 summed, bf16 and f32), forward and dw, what they choose is 0.4 % slower than the
 // better of the two in the mean, at most 15 %: 3 328 x 3 328 x 2 048 bf16 256 46 us (128: 68), 3 297 x 1 483 x 2 048 bf16 128 41 (256: 48), 2 304 x 2 304 x 4 096 bf16 256 62
 // (128: 76), 6 000 x 3 003 x 1 001 f32 128 345 (256: 513).
 static Plan plan_product(int64_t ri, int64_t rj, int64_t depth, int dtype) {
