@@ -152,20 +152,28 @@ variable_list no_second(const char* name, variable_list&& grads, std::initialize
   return std::move(grads);
 }
 
-// the capture that the device's current stream takes part in: a number that no other capture has, or 0
-uint64_t capture_on(at::Device dev) {
+// the capture that a stream takes part in: a number that no other capture has, or 0
+uint64_t capture_of(hipStream_t stream) {
   hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
   unsigned long long id = 0;
-  C10_HIP_CHECK(hipStreamGetCaptureInfo(c10::hip::getCurrentHIPStream(dev.index()).stream(), &status, &id));
+  C10_HIP_CHECK(hipStreamGetCaptureInfo(stream, &status, &id));
   return status == hipStreamCaptureStatusNone ? 0 : id;
 }
+uint64_t capture_on(at::Device dev) { return capture_of(c10::hip::getCurrentHIPStream(dev.index()).stream()); }
 
 // A captured step must not meet an eager graph of the same leaves that is still alive, or go on from one: the leaves' gradient nodes (or that graph's own) belong to the
 // stream that it was recorded on, the backward pass would wait on that stream from inside the capture, and torch ends the process there.  Said here, where it can
 // still be said, of everything that the inputs were made from.
 void refuse_capture_beside_eager(at::Device dev, std::initializer_list<const Tensor*> inputs) {
-  if (!capture_on(dev)) return;
+  const uint64_t capture = capture_on(dev);
+  if (!capture) return;
   const auto here = c10::hip::getCurrentHIPStream(dev.index()).id();
+  // (a stream that has joined the capture belongs to it; the null stream never does, and may not be asked)
+  auto inside = [&](const c10::Stream& s) {
+    if (s.id() == here) return true;
+    const hipStream_t stream = c10::hip::HIPStream(c10::hip::HIPStream::UNCHECKED, s).stream();
+    return stream && capture_of(stream) == capture;
+  };
   std::vector<std::shared_ptr<Node>> todo;
   std::unordered_set<Node*> seen;
   for (const Tensor* t : inputs) {
@@ -178,7 +186,7 @@ void refuse_capture_beside_eager(at::Device dev, std::initializer_list<const Ten
     todo.pop_back();
     if (!seen.insert(node.get()).second) continue;
     const auto at = node->stream();
-    if (at && at->id() != here)
+    if (at && !inside(*at))
       refuse("a tensor that requires a gradient is still part of a graph recorded outside of this capture: drop that graph's results before capturing");
     for (const auto& edge : node->next_edges())
       if (edge.function) todo.push_back(edge.function);

@@ -529,8 +529,6 @@ class MiniGridVecEnv(_VectorEnvBase):
             log_prob = torch.empty((steps, n), dtype=torch.float32, device=dev)
             value = torch.empty((steps, n), dtype=torch.float32, device=dev)
             final = torch.zeros((steps, n), dtype=torch.float32, device=dev) if final_value else None
-            u = torch.rand((steps, n), generator=torch.Generator(dev).manual_seed(_draw_seed(action_seed, self._draws, self.env_index_base)), device=dev)
-            self._draws += steps
             done = None
             if self._slot0 != "step":
                 done = torch.from_numpy(self.get_state()[1][:, 6] != 0)                   # (whose reset is due)
@@ -541,6 +539,8 @@ class MiniGridVecEnv(_VectorEnvBase):
                     B.check(self._lib.mg_reset(self._h, None, self._p(np.zeros(n, np.uint8))), self._h)
             done = (out["terminated"] | out["truncated"]).bool() if done is None or mode != "next_step" else done.to(dev)
             self._slot0 = "step"
+            u = torch.rand((steps, n), generator=torch.Generator(dev).manual_seed(_draw_seed(action_seed, self._draws, self.env_index_base)), device=dev)
+            self._draws += steps
             obs = self._collect()[0]
             for t in range(steps):
                 image[t].copy_(out["image"])

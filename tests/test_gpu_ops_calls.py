@@ -472,3 +472,23 @@ def test_capture_of_what_was_made_from_leaves_of_an_eager_graph_is_refused(op):
     g.replay()
     torch.cuda.synchronize()
     assert torch.equal(d, torch.autograd.grad(step(), [x])[0])
+
+
+def test_capture_over_two_streams():
+    """a stream that has joined the capture is part of it: what was recorded there is no eager graph"""
+    x = torch.randn((40, 7), generator=gen(1), device="cuda", requires_grad=True)
+    w, v = (torch.randn((7, 7), generator=gen(i), device="cuda", requires_grad=True) for i in (2, 3))
+    want = mg().linear(mg().linear(x, w, activation="tanh"), v).detach().clone()
+    torch.cuda.synchronize()
+    side, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            h = mg().linear(x, w, activation="tanh")
+        torch.cuda.current_stream().wait_stream(side)
+        y = mg().linear(h, v)
+    for _ in range(3):
+        y.detach().zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want)
