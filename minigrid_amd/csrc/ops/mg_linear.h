@@ -103,6 +103,7 @@ __device__ __forceinline__ float activate(int act, float z) {
   }
 }
 
+// (An infinite z is one that did not fit 16 bits: the slope there is the limit, 0 or 1, not infinity times 0.  Beyond the bounds that z is held in the other factor is 0.)
 __device__ __forceinline__ float activate_grad(int act, float z) {
   switch (act) {
     case MG_ACTIVATION_RELU: return z > 0.0f ? 1.0f : (z != z ? z : 0.0f);
@@ -113,11 +114,11 @@ __device__ __forceinline__ float activate_grad(int act, float z) {
     case MG_ACTIVATION_GELU: {
       float d;
       const float t = phi_tail(fabsf(z), &d);
-      return (z < 0.0f ? t : 1.0f - t) + z * d;
+      return (z < 0.0f ? t : 1.0f - t) + fminf(fmaxf(z, -16.0f), 16.0f) * d;        // (a NaN is in t)
     }
     case MG_ACTIVATION_SILU: {
       const float p = rcp_fast(1.0f + exp2_fast(z * -1.44269504f));
-      return p * __builtin_fmaf(z, 1.0f - p, 1.0f);
+      return p * __builtin_fmaf(fminf(fmaxf(z, -200.0f), 200.0f), 1.0f - p, 1.0f);  // (a NaN is in p)
     }
     default: return 1.0f;
   }

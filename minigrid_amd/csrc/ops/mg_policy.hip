@@ -355,7 +355,7 @@ __device__ __forceinline__ Saved row_result(const LossArgs& a, int64_t i, const 
 // The sums of a long row are made in 32 bits: d = l - m is rounded (2^-24 |d|), so is d log2 e (2^-24 |d|, and its constant another 1.4e-8 |d|), the exponential is
 // good to 2^-23, and up to eight terms are added in 32 bits (7 x 2^-24).  So s, and with it the ratio, is off by at most 2^-24 (9 + 2.3 D) of itself, D = -t / s
 // the mean of |d| under the row's distribution.  Where that leaves open whether the ratio is beyond its border (a row in 10^5 or so), the row's first wave sums
-// it again with 64-bit exponentials.
+// it again with 64-bit exponentials.  (Where every row lies on its border, a clip of 0 and a policy that has not moved, 16 384 x 40 961 bf16 take 3.2 ms.)
 __device__ __forceinline__ double sums_error(double s, double t) { return 0x1p-24 * (16.0 - 4.0 * (t / s)); }
 struct Sums64 { double s, t; };
 template <class T>

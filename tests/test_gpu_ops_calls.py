@@ -492,3 +492,29 @@ def test_capture_over_two_streams():
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("act", ["gelu", "silu", "tanh", "relu"])
+@pytest.mark.parametrize("rows", [3, 40, 300])
+def test_linear_slope_beyond_the_largest_half(act, rows):
+    """values in front of the activation that do not fit 16 bits: far on the negative side the result is 0 and so is the slope, on the positive side the slope is 1 (tanh: 0)"""
+    k, n = 64, 72
+    x = torch.full((rows, k), 100.0, dtype=torch.float16, device="cuda")
+    w = torch.full((n, k), -100.0, dtype=torch.float16, device="cuda")
+    w[1::2] = 100.0                                                  # z = -640 000 and 640 000
+    x, w = x.requires_grad_(True), w.requires_grad_(True)
+    b = torch.zeros(n, dtype=torch.float16, device="cuda", requires_grad=True)
+    r = torch.zeros((rows, n), dtype=torch.float16, device="cuda")
+    for res in (None, r):
+        y = mg().linear(x, w, b, activation=act, residual=res)
+        dy = torch.full_like(y, 2.0 ** -10)
+        dx, dw, db = torch.autograd.grad(y, [x, w, b], dy)
+        slope = 0.0 if act == "tanh" else 1.0
+        if act != "tanh":
+            assert not bool(y[:, ::2].any()) and bool(y[:, 1::2].isinf().all())
+        assert not bool(db[::2].any()) and not bool(dw[::2].any())
+        # (powers of two and small whole numbers of them: exact up to 2 048 of the smallest)
+        assert torch.equal(db[1::2].double(), torch.full((n // 2,), rows * slope * 2.0 ** -10, dtype=torch.float64, device="cuda"))
+        want = dw[1::2].double() - rows * slope * 100 * 2.0 ** -10
+        assert float(want.abs().max()) <= half(torch.float16) * rows * 100 * 2.0 ** -10
+        assert torch.equal(dx.double(), torch.full((rows, k), 36 * slope * 100 * 2.0 ** -10, dtype=torch.float64, device="cuda").half().double())
