@@ -518,3 +518,19 @@ def test_linear_slope_beyond_the_largest_half(act, rows):
         want = dw[1::2].double() - rows * slope * 100 * 2.0 ** -10
         assert float(want.abs().max()) <= half(torch.float16) * rows * 100 * 2.0 ** -10
         assert torch.equal(dx.double(), torch.full((rows, k), 36 * slope * 100 * 2.0 ** -10, dtype=torch.float64, device="cuda").half().double())
+
+
+def test_rollout_behind_a_changed_observation():
+    """an observation wrapper changes what the env shows: the first observation of a rollout is the new one"""
+    envs, twin = (toy_envs(48, "MiniGrid-DoorKey-5x5-v0", max_steps=20) for _ in range(2))
+    twin = mg().FullyObsWrapper(twin)
+    envs.reset(seed=3)
+    obs, _ = twin.reset(seed=3)
+    image = obs["image"].clone()
+    envs = mg().FullyObsWrapper(envs)
+    got, want = envs.rollout(6, policy=toy_policy), twin.rollout(6, policy=toy_policy)
+    assert torch.equal(got.image[0], image)
+    for name in ("image", "direction", "mission_id", "action", "value", "reward", "done"):
+        assert torch.equal(getattr(got, name), getattr(want, name)), name
+    envs.close()
+    twin.close()

@@ -82,3 +82,10 @@ def test_assembly_names_the_special_registers_that_it_writes():
                     found += 1
                     assert '"%s"' % reg in text.split(":")[-1], (os.path.basename(path), text)
     assert found
+
+
+def test_seeds_of_rollouts_are_their_own():
+    from minigrid_amd.vector_env import _draw_seed
+    assert _draw_seed(7, 0, 0) == 7 and _draw_seed(-3, 0, 0) == -3
+    seen = {_draw_seed(s, t, b) for s in (0, 1, 2, -1, 2 ** 63) for t in (0, 1, 2, 128, 256, 2 ** 31) for b in (0, 1, 64, 2 ** 20)}
+    assert len(seen) == 5 * 6 * 4 and all(-2 ** 63 <= v < 2 ** 64 for v in seen)
