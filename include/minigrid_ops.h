@@ -22,18 +22,19 @@ extern "C" {
 #endif
 
 typedef enum mg_dtype { MG_DT_F32 = 0, MG_DT_BF16 = 1, MG_DT_F16 = 2, MG_DT_U8 = 3, MG_DT_F64 = 4, MG_DT_I32 = 5, MG_DT_I64 = 6 } mg_dtype;
-typedef enum mg_activation { MG_ACTIVATION_NONE = 0, MG_ACTIVATION_RELU = 1, MG_ACTIVATION_TANH = 2, MG_ACTIVATION_GELU = 3, MG_ACTIVATION_SILU = 4 } mg_activation;
+typedef enum mg_activation { MG_ACTIVATION_NONE = 0, MG_ACTIVATION_RELU = 1, MG_ACTIVATION_TANH = 2, MG_ACTIVATION_GELU = 3, MG_ACTIVATION_SILU = 4,
+  MG_ACTIVATION_TANH_Z32 = 18 /* tanh whose z is f32 whatever the dtype: from a z rounded to 16 bits its slope loses the most */ } mg_activation;
 
 MG_API const char* mg_ops_last_error(void);
 
 /* ---- a layer of a policy network: y = act(x wT + b) + r ----
  * x (rows, k) of `dtype` or bytes (x_dtype = MG_DT_U8: an observation as the environments write it), w (n, k), b (n) or NULL, r (rows, n) or NULL,
- * y (rows, n), all of `dtype` (f32, bf16, f16).  z (rows, n, contiguous; `dtype`, for tanh f32) or NULL: the values in front of the activation, for the
- * backward pass.  Sums are held in 32 bits.  act = gelu is x Phi(x) with the normal distribution function itself. */
+ * y (rows, n), all of `dtype` (f32, bf16, f16).  z (rows, n, contiguous; `dtype`, f32 for MG_ACTIVATION_TANH_Z32) or NULL: the values in front of the
+ * activation, for the backward pass.  Sums are held in 32 bits.  act = gelu is x Phi(x) with the normal distribution function itself. */
 MG_API int mg_op_linear_workspace(int64_t rows, int64_t k, int64_t n, int dtype, int64_t* forward, int64_t* backward_input, int64_t* backward_weight);
 MG_API int mg_op_linear(int device, void* stream, int dtype, int x_dtype, int act, int64_t rows, int64_t k, int64_t n, const void* x, int64_t ldx,
                         const void* w, int64_t ldw, const void* b, const void* r, int64_t ldr, void* y, int64_t ldy, void* z, void* ws, int64_t ws_bytes);
-/* dz = dy * act'(z), z as the forward pass has left it (dz: rows, n, contiguous; NULL allowed for act = none) and db = the column sums of dz (n, `dtype`; NULL = not wanted).
+/* dz = dy * act'(z), z as a forward pass with the same act has left it (dz: rows, n, contiguous; NULL allowed for act = none) and db = the column sums of dz (n, `dtype`; NULL = not wanted).
  * ws: mg_op_linear_dz_workspace bytes (needed for db only). */
 MG_API int mg_op_linear_dz_workspace(int64_t rows, int64_t n, int64_t* bytes);
 MG_API int mg_op_linear_dz(int device, void* stream, int dtype, int act, int64_t rows, int64_t n, const void* dy, int64_t lddy, const void* z, void* dz,

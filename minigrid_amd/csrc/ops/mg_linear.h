@@ -49,10 +49,10 @@ struct Epilogue {
 
 // ---- activations ----
 // What a backward pass keeps of z.  For most activations z in the operands' type: the slope at a rounded z is off by less than dz's own rounding (by a third of it for
-// gelu and silu at z of 1).  tanh's slope falls as e^{-2 |z|}, so at a rounded z it would be off by 2 |z| half steps of itself: z stays in 32 bits.  (dx and
+// gelu and silu at z of 1).  tanh's slope falls as e^{-2 |z|}, so at a rounded z it is off by 2 |z| half steps of itself: for MG_ACTIVATION_TANH_Z32 z stays in 32 bits.  (dx and
 // dw of 2 049 x 300 x 136 bf16 are off by 2.55e-3 of their norm with a rounded z, 2.33e-3 without, by 1.66e-3 where they alone are rounded; the forward and backward
 // pass of 65 536 x 512 x 512 take 238 and 253 us.)
-template <class T, int ACT> using KeptOf = std::conditional_t<ACT == MG_ACTIVATION_TANH, float, T>;
+template <class T, int ACT> using KeptOf = std::conditional_t<ACT == MG_ACTIVATION_TANH_Z32, float, T>;
 
 // exp2 with a result of 0 far below the smallest number: v_exp_f32, one ulp
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -92,7 +92,7 @@ __device__ __forceinline__ float tanh_act(float z) {
 __device__ __forceinline__ float activate(int act, float z) {
   switch (act) {
     case MG_ACTIVATION_RELU: return z < 0.0f ? 0.0f : z;                       // (keeps a NaN)
-    case MG_ACTIVATION_TANH: return tanh_act(z);
+    case MG_ACTIVATION_TANH: case MG_ACTIVATION_TANH_Z32: return tanh_act(z);
     case MG_ACTIVATION_GELU: {
       float d;
       const float t = phi_tail(fabsf(z), &d);
@@ -107,7 +107,7 @@ __device__ __forceinline__ float activate(int act, float z) {
 __device__ __forceinline__ float activate_grad(int act, float z) {
   switch (act) {
     case MG_ACTIVATION_RELU: return z > 0.0f ? 1.0f : (z != z ? z : 0.0f);
-    case MG_ACTIVATION_TANH: {
+    case MG_ACTIVATION_TANH: case MG_ACTIVATION_TANH_Z32: {
       const float t = tanh_act(z), e = exp2_fast(fabsf(z) * (-2.0f * 1.44269504f)), q = rcp_fast(1.0f + e);
       return fabsf(z) < 0.3f ? 1.0f - t * t : 4.0f * e * q * q;                // 1 - tanh^2 = 4 e^{-2|z|} / (1 + e^{-2|z|})^2
     }
@@ -277,7 +277,7 @@ template <class T>
 __device__ __forceinline__ void finish(const Epilogue& e, int64_t i, int64_t j, int64_t n, float v) {
   if (e.b) v += (float)((const T*)e.b)[j];
   if (e.z) {
-    if (e.act == MG_ACTIVATION_TANH) ((float*)e.z)[i * n + j] = v;
+    if (e.act == MG_ACTIVATION_TANH_Z32) ((float*)e.z)[i * n + j] = v;
     else ((T*)e.z)[i * n + j] = (T)v;
   }
   v = activate(e.act, v);
@@ -531,6 +531,9 @@ __device__ __forceinline__ void store_wave_any(const Epilogue& ep, f32x16 (&acc)
     switch (ep.part ? MG_ACTIVATION_NONE : ep.act) {
       case MG_ACTIVATION_RELU: MG_ACT(MG_ACTIVATION_RELU); return;
       case MG_ACTIVATION_TANH: MG_ACT(MG_ACTIVATION_TANH); return;
+      case MG_ACTIVATION_TANH_Z32:                               // (32-bit operands: the same as tanh, which is asked for)
+        if constexpr (sizeof(T) == 2) { MG_ACT(MG_ACTIVATION_TANH_Z32); }
+        return;
       case MG_ACTIVATION_GELU: MG_ACT(MG_ACTIVATION_GELU); return;
       case MG_ACTIVATION_SILU: MG_ACT(MG_ACTIVATION_SILU); return;
       default: MG_ACT(MG_ACTIVATION_NONE); return;
@@ -548,6 +551,9 @@ __device__ __forceinline__ void store_tile_any(const Epilogue& ep, f32x16 (&acc)
     switch (ep.part ? MG_ACTIVATION_NONE : ep.act) {
       case MG_ACTIVATION_RELU: MG_ACT(MG_ACTIVATION_RELU); return;
       case MG_ACTIVATION_TANH: MG_ACT(MG_ACTIVATION_TANH); return;
+      case MG_ACTIVATION_TANH_Z32:                               // (32-bit operands: the same as tanh, which is asked for)
+        if constexpr (sizeof(T) == 2) { MG_ACT(MG_ACTIVATION_TANH_Z32); }
+        return;
       case MG_ACTIVATION_GELU: MG_ACT(MG_ACTIVATION_GELU); return;
       case MG_ACTIVATION_SILU: MG_ACT(MG_ACTIVATION_SILU); return;
       default: break;

@@ -84,6 +84,10 @@ static int product(hipStream_t st, int form, bool bytes, const Operand& A, const
   });
 }
 
+static bool known(int act) { return (act >= MG_ACTIVATION_NONE && act <= MG_ACTIVATION_SILU) || act == MG_ACTIVATION_TANH_Z32; }
+// (a z of 32-bit operands is f32 either way)
+static int kernel_act(int act, int dtype) { return act == MG_ACTIVATION_TANH_Z32 && dtype == MG_DT_F32 ? MG_ACTIVATION_TANH : act; }
+
 static int check_sizes(int64_t rows, int64_t k, int64_t n, int dtype) {
   if (dtype != MG_DT_F32 && dtype != MG_DT_BF16 && dtype != MG_DT_F16) return fail(MG_ERR_INVALID, "dtype must be f32, bf16 or f16");
   if (rows < 0 || k < 1 || n < 1 || rows > 0x7fffff00ll || k > 0x7fffff00ll || n > 0x7fffff00ll) return fail(MG_ERR_INVALID, "sizes must be 0 <= rows, 1 <= k, 1 <= n, below 2^31 - 256");
@@ -110,14 +114,14 @@ int mg_op_linear(int device, void* stream, int dtype, int x_dtype, int act, int6
   int rc = check_sizes(rows, k, n, dtype);
   if (rc != MG_OK) return rc;
   if (x_dtype != dtype && x_dtype != MG_DT_U8) return fail(MG_ERR_INVALID, "x must have w's type or be bytes");
-  if (act < MG_ACTIVATION_NONE || act > MG_ACTIVATION_SILU) return fail(MG_ERR_INVALID, "unknown activation %d", act);
+  if (!known(act)) return fail(MG_ERR_INVALID, "unknown activation %d", act);
   if (rows == 0) return MG_OK;
   if (!x || !w || !y) return fail(MG_ERR_INVALID, "x, w and y must not be NULL");
   if (ldx < k || ldw < k || ldy < n || (r && ldr < n)) return fail(MG_ERR_INVALID, "a row stride is smaller than its row");
   DeviceGuard g(device);
   if (g.rc != MG_OK) return g.rc;
   hipStream_t st = (hipStream_t)stream;
-  Epilogue ep = {b, r, y, z, nullptr, ldr, ldy, act, 0};
+  Epilogue ep = {b, r, y, z, nullptr, ldr, ldy, kernel_act(act, dtype), 0};
   const bool bytes = x_dtype == MG_DT_U8;
   if (rows <= FEW_ROWS)
     return by_type(dtype, [&](auto* t) {
@@ -138,7 +142,7 @@ int mg_op_linear_dz(int device, void* stream, int dtype, int act, int64_t rows, 
                     void* ws, int64_t ws_bytes) {
   int rc = check_sizes(rows, 1, n, dtype);
   if (rc != MG_OK) return rc;
-  if (act < MG_ACTIVATION_NONE || act > MG_ACTIVATION_SILU) return fail(MG_ERR_INVALID, "unknown activation %d", act);
+  if (!known(act)) return fail(MG_ERR_INVALID, "unknown activation %d", act);
   if (act != MG_ACTIVATION_NONE && !z && rows) return fail(MG_ERR_INVALID, "the values in front of the activation are needed");
   if ((!dy && rows) || lddy < n) return fail(MG_ERR_INVALID, "dy must not be NULL and its row stride not smaller than its row");
   DeviceGuard g(device);
@@ -149,7 +153,7 @@ int mg_op_linear_dz(int device, void* stream, int dtype, int act, int64_t rows, 
   if (db && (need > ws_bytes || !ws || ((uintptr_t)ws & 255))) return fail(MG_ERR_INVALID, "workspace: %lld bytes, 256-byte aligned, are needed", (long long)need);
   if (p.strips > 0x7fffffffll || p.runs > 65535) return fail(MG_ERR_INVALID, "too many rows or columns");
   return by_type(dtype, [&](auto* t) {
-    Linear<std::remove_pointer_t<decltype(t)>>::dz(st, act, rows, n, dy, lddy, z, dz, db, db ? (float*)ws : nullptr);
+    Linear<std::remove_pointer_t<decltype(t)>>::dz(st, kernel_act(act, dtype), rows, n, dy, lddy, z, dz, db, db ? (float*)ws : nullptr);
     return launched("dz");
   });
 }

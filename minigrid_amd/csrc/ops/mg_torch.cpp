@@ -304,7 +304,8 @@ Tensor linear(const Tensor& x, const Tensor& w, const MaybeTensor& bias, int64_t
     const int64_t rows = xm.size(0);
     const int dt = dtype_of(type);
     y = make(shape, type, dev);
-    if (node && act && !from_y) z = make({rows, n}, act == MG_ACTIVATION_TANH ? at::kFloat : type, dev);
+    if (node && act == MG_ACTIVATION_TANH) act = MG_ACTIVATION_TANH_Z32;
+    if (node && act && !from_y) z = make({rows, n}, act == MG_ACTIVATION_TANH_Z32 ? at::kFloat : type, dev);
     int64_t need = 0;
     check(L.mg_op_linear_workspace(rows, k, n, dt, &need, nullptr, nullptr));
     const Scratch ws(need, dev);

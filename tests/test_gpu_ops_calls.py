@@ -534,3 +534,32 @@ def test_rollout_behind_a_changed_observation():
         assert torch.equal(getattr(got, name), getattr(want, name)), name
     envs.close()
     twin.close()
+
+
+@pytest.mark.parametrize("act,kept", [(2, torch.bfloat16), (18, torch.float32)])
+@pytest.mark.parametrize("rows,k,n", [(3, 30, 33), (40, 30, 33), (40, 4096, 130), (300, 513, 257), (4104, 1032, 2056)])
+def test_c_entry_keeps_z_as_the_header_says(act, kept, rows, k, n):
+    """tanh's z in the operands' type, or in 32 bits for MG_ACTIVATION_TANH_Z32: no byte behind (rows, n) of it is written, and the slope is told from it"""
+    import ctypes as C
+
+    from minigrid_amd import ops
+    L = ops._lib()
+    x, w, b, _, dy = linear_inputs(rows, k, n, torch.bfloat16, False, True, False, False, 3)
+    z = torch.full((rows * n + 4096,), -7.0, dtype=kept, device="cuda")
+    y, dz = torch.empty((rows, n), dtype=torch.bfloat16, device="cuda"), torch.empty((rows, n), dtype=torch.bfloat16, device="cuda")
+    need = C.c_int64()
+    assert L.mg_op_linear_workspace(rows, k, n, 1, C.byref(need), None, None) == 0
+    ws = torch.empty(need.value + 256, dtype=torch.uint8, device="cuda")
+    st = torch.cuda.current_stream().cuda_stream
+    p = lambda t: t.data_ptr()
+    assert L.mg_op_linear(0, st, 1, 1, act, rows, k, n, p(x), k, p(w), k, p(b), None, 0, p(y), n, p(z), p(ws), need.value) == 0, L.mg_ops_last_error()
+    assert L.mg_op_linear_dz(0, st, 1, act, rows, n, p(dy), n, p(z), p(dz), None, None, 0) == 0, L.mg_ops_last_error()
+    torch.cuda.synchronize()
+    assert bool((z[rows * n:] == -7.0).all())
+    Z = x.double() @ w.double().t() + b.double()
+    ez = (k + 4) * U * (x.double().abs() @ w.double().abs().t() + b.double().abs())
+    within(z[:rows * n].view(rows, n), Z, 1.01 * ez + half(kept) * Z.abs() * 1.01 + 1e-30, "z")
+    kz = z[:rows * n].view(rows, n).double()
+    want = dy.double() * (1 - torch.tanh(kz) ** 2)
+    within(dz, want, 4 * EL * want.abs() + half(torch.bfloat16) * 1.01 * want.abs() + 1e-30, "dz")
+    assert L.mg_op_linear(0, st, 1, 1, 17, rows, k, n, p(x), k, p(w), k, p(b), None, 0, p(y), n, p(z), p(ws), need.value) != 0
